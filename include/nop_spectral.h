@@ -399,6 +399,48 @@ int32_t nop_tucker_grads(int32_t n, const int64_t* dims, const int64_t* ranks, c
                          const void* const* factors, const void* grad_w, void* grad_core, void* const* grad_factors,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- per-point norm -------------------------------------------------------------------------
+ * Root-mean-square norm over the channels of every point of a field [batch, channels, points]:
+ *   r = x + residual (rounded to the field's type; r = x without a residual),
+ *   y_c = r_c / sqrt(mean_c r_c^2 + eps) * weight_c.
+ * weight: [channels] float32, or NULL for ones.  The statistics are fp32. */
+typedef enum nop_dtype { NOP_DTYPE_FP32 = 0, NOP_DTYPE_BF16 = 1, NOP_DTYPE_FP16 = 2, NOP_DTYPE_E4M3 = 3 } nop_dtype;
+
+typedef struct nop_norm_desc {
+    int32_t abi_version;
+    int32_t dtype;        /* nop_dtype of x, residual, y, r and their gradients: fp32, bf16 or fp16 */
+    int64_t batch;        /* >= 0 */
+    int64_t points;       /* per sample, >= 0 */
+    int32_t channels;     /* 1..8192 */
+    float eps;            /* >= 0 */
+} nop_norm_desc;
+
+/* residual and r are given together or not at all.  Either y is written, or q and scale: q = e4m3(y / s), one
+ * byte a value, and scale [batch, points] float32 = s, for every point the least power of two with
+ * max_c |y_c| <= 448 s (1 where all are zero or one is not finite; at least 2^-126). */
+int32_t nop_rms_norm_forward(const nop_norm_desc* desc, const void* x, const void* residual, const float* weight,
+                             void* y, void* r, void* q, float* scale, void* stream);
+
+/* gx = dL/dr (which is both dL/dx and dL/dresidual) from gy = dL/dy and, when r was used beside y, gr (or NULL);
+ * gw = dL/dweight [channels] float32.  gx or gw may be NULL.  r: the forward's sum (x without a residual).
+ * workspace: needed for gw; the sums over the points are added in a fixed order. */
+int32_t nop_rms_norm_backward_workspace_size(const nop_norm_desc* desc, size_t* bytes);
+int32_t nop_rms_norm_backward(const nop_norm_desc* desc, const void* r, const float* weight, const void* gy,
+                              const void* gr, void* gx, float* gw, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* ---- global norm over many tensors, and clipping ---------------------------------------------
+ * norm = sqrt(sum of squares over all n tensors) (NOP_NORM_L2) or the largest magnitude (NOP_NORM_INF), left in
+ * *norm (device float32, may be NULL when dst is given); dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)), with
+ * dst[i] == src[i] for clipping in place (nothing is written then when the factor is 1), or dst = NULL for the norm
+ * alone.  numel: values of each tensor (two for a complex one); dtypes: fp32, bf16 or fp16 for each.  Tensors must
+ * not overlap one another.  No host synchronisation; the sums do not depend on scheduling. */
+typedef enum nop_norm_type { NOP_NORM_L2 = 0, NOP_NORM_INF = 1 } nop_norm_type;
+int32_t nop_clip_workspace_size(int32_t n, size_t* bytes);
+int32_t nop_clip_by_norm(int32_t n, const void* const* src, void* const* dst, const int64_t* numel,
+                         const int32_t* dtypes, int32_t norm_type, double max_norm, float* norm, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,10 +35,14 @@ EXPORTED_SYMBOLS = (
     "nop_device_status", "nop_chain_query", "nop_chain_forward", "nop_chain_backward_query", "nop_chain_backward",
     "nop_spectral_spectrum_layout", "nop_spectral_forward_keep", "nop_spectral_weight_grad",
     "nop_spectral_weight_grad_workspace_size", "nop_spectral_pack_weights_adjoint",
-    "nop_tucker_grads_workspace_size", "nop_tucker_grads",
+    "nop_tucker_grads_workspace_size", "nop_tucker_grads", "nop_rms_norm_forward",
+    "nop_rms_norm_backward_workspace_size", "nop_rms_norm_backward", "nop_clip_workspace_size", "nop_clip_by_norm",
 )
 
 MAX_SLAB_RANKS = 64
+
+DTYPE_FP32, DTYPE_BF16, DTYPE_FP16, DTYPE_E4M3 = 0, 1, 2, 3
+NORM_L2, NORM_INF = 0, 1
 
 
 class NopSpectralDesc(ctypes.Structure):
@@ -83,6 +87,17 @@ class NopSlabInfo(ctypes.Structure):
         ("recv1_split", ctypes.c_size_t * 64),
         ("send2_split", ctypes.c_size_t * 64),
         ("recv2_split", ctypes.c_size_t * 64),
+    ]
+
+
+class NopNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("points", ctypes.c_int64),
+        ("channels", ctypes.c_int32),
+        ("eps", ctypes.c_float),
     ]
 
 
@@ -161,6 +176,19 @@ def _declare(lib):
         ctypes.c_int32, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p,
         ctypes.POINTER(ctypes.c_void_p), ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p),
         ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    vp, size = ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)
+    lib.nop_rms_norm_forward.restype = ctypes.c_int32
+    lib.nop_rms_norm_forward.argtypes = [ctypes.POINTER(NopNormDesc)] + [vp] * 8
+    lib.nop_rms_norm_backward_workspace_size.restype = ctypes.c_int32
+    lib.nop_rms_norm_backward_workspace_size.argtypes = [ctypes.POINTER(NopNormDesc), size]
+    lib.nop_rms_norm_backward.restype = ctypes.c_int32
+    lib.nop_rms_norm_backward.argtypes = [ctypes.POINTER(NopNormDesc)] + [vp] * 7 + [ctypes.c_size_t, vp]
+    lib.nop_clip_workspace_size.restype = ctypes.c_int32
+    lib.nop_clip_workspace_size.argtypes = [ctypes.c_int32, size]
+    lib.nop_clip_by_norm.restype = ctypes.c_int32
+    lib.nop_clip_by_norm.argtypes = [
+        ctypes.c_int32, ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_int64),
+        ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, ctypes.c_double, vp, vp, ctypes.c_size_t, vp]
     lib.nop_device_status.restype = ctypes.c_int32
     lib.nop_device_status.argtypes = [ctypes.POINTER(ctypes.c_int32), ctypes.c_int32]
     lib.nop_spectral_host_workspace_size.restype = ctypes.c_int32
@@ -233,6 +261,19 @@ def last_error() -> str:
 
 
 def check(code: int):
+    if code != NOP_OK:
+        raise NopError(code, last_error())
+
+
+def call(fn, device, *args):
+    """fn(*args, stream) on ``device`` (a torch CUDA device) and its current stream, its status checked."""
+    import torch
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        code = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, stream)
     if code != NOP_OK:
         raise NopError(code, last_error())
 
