@@ -429,6 +429,61 @@ int32_t nop_rms_norm_backward(const nop_norm_desc* desc, const void* r, const fl
                               const void* gr, void* gx, float* gw, void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/* ---- gated feed-forward block ----------------------------------------------------------------
+ * At every point of x [batch, channels, points]:
+ *   h = act(w_gate x + b_gate) * (w_up x + b_up),  y = w_down h + b_down      y [batch, out_channels, points]
+ * w_gate, w_up [hidden, channels], w_down [out_channels, hidden], biases (each may be NULL) [hidden], [hidden],
+ * [out_channels], all of the field's type `dtype`.  fp32 in fp32 accuracy; 16-bit types with fp32 sums, h rounded
+ * to the type.  x_dtype: dtype, or NOP_DTYPE_E4M3 (forward only, 16-bit dtype) with x_scale [batch, points]
+ * float32, the values being x * x_scale.  Values that are not finite give results that are not finite at their
+ * point.  channels and out_channels <= 256, hidden <= 16384, fewer than 2^31 points. */
+typedef enum nop_activation { NOP_ACT_SILU = 0, NOP_ACT_GELU = 1 } nop_activation;
+
+typedef struct nop_gated_desc {
+    int32_t abi_version;
+    int32_t dtype;
+    int32_t x_dtype;
+    int32_t activation;
+    int64_t batch;
+    int64_t points;
+    int32_t channels;
+    int32_t hidden;
+    int32_t out_channels;
+    int32_t reserved;
+} nop_gated_desc;
+
+typedef struct nop_gated_operands {
+    const void* x;
+    const float* x_scale;
+    const void* w_gate;
+    const void* w_up;
+    const void* w_down;
+    const void* b_gate;
+    const void* b_up;
+    const void* b_down;
+    void* y;                /* forward only */
+} nop_gated_operands;
+
+/* Gradients, of the operands' types and shapes; each but gy (dL/dy) may be NULL.  The forward's intermediates are
+ * computed again from x; sums over the points are added in a fixed order. */
+typedef struct nop_gated_grads {
+    const void* gy;
+    void* gx;
+    void* gw_gate;
+    void* gw_up;
+    void* gw_down;
+    void* gb_gate;
+    void* gb_up;
+    void* gb_down;
+} nop_gated_grads;
+
+/* workspace: device memory, 256-byte aligned, of the size for the pass (backward: 0 or 1). */
+int32_t nop_gated_workspace_size(const nop_gated_desc* desc, int32_t backward, size_t* bytes);
+int32_t nop_gated_forward(const nop_gated_desc* desc, const nop_gated_operands* operands, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int32_t nop_gated_backward(const nop_gated_desc* desc, const nop_gated_operands* operands, const nop_gated_grads* grads,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- global norm over many tensors, and clipping ---------------------------------------------
  * norm = sqrt(sum of squares over all n tensors) (NOP_NORM_L2) or the largest magnitude (NOP_NORM_INF), left in
  * *norm (device float32, may be NULL when dst is given); dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)), with

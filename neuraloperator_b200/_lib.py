@@ -37,12 +37,14 @@ EXPORTED_SYMBOLS = (
     "nop_spectral_weight_grad_workspace_size", "nop_spectral_pack_weights_adjoint",
     "nop_tucker_grads_workspace_size", "nop_tucker_grads", "nop_rms_norm_forward",
     "nop_rms_norm_backward_workspace_size", "nop_rms_norm_backward", "nop_clip_workspace_size", "nop_clip_by_norm",
+    "nop_gated_workspace_size", "nop_gated_forward", "nop_gated_backward",
 )
 
 MAX_SLAB_RANKS = 64
 
 DTYPE_FP32, DTYPE_BF16, DTYPE_FP16, DTYPE_E4M3 = 0, 1, 2, 3
 NORM_L2, NORM_INF = 0, 1
+ACT_SILU, ACT_GELU = 0, 1
 
 
 class NopSpectralDesc(ctypes.Structure):
@@ -99,6 +101,31 @@ class NopNormDesc(ctypes.Structure):
         ("channels", ctypes.c_int32),
         ("eps", ctypes.c_float),
     ]
+
+
+class NopGatedDesc(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("points", ctypes.c_int64),
+        ("channels", ctypes.c_int32),
+        ("hidden", ctypes.c_int32),
+        ("out_channels", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class NopGatedOperands(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in
+                ("x", "x_scale", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down", "y")]
+
+
+class NopGatedGrads(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in
+                ("gy", "gx", "gw_gate", "gw_up", "gw_down", "gb_gate", "gb_up", "gb_down")]
 
 
 class NopError(RuntimeError):
@@ -183,6 +210,14 @@ def _declare(lib):
     lib.nop_rms_norm_backward_workspace_size.argtypes = [ctypes.POINTER(NopNormDesc), size]
     lib.nop_rms_norm_backward.restype = ctypes.c_int32
     lib.nop_rms_norm_backward.argtypes = [ctypes.POINTER(NopNormDesc)] + [vp] * 7 + [ctypes.c_size_t, vp]
+    lib.nop_gated_workspace_size.restype = ctypes.c_int32
+    lib.nop_gated_workspace_size.argtypes = [ctypes.POINTER(NopGatedDesc), ctypes.c_int32, size]
+    lib.nop_gated_forward.restype = ctypes.c_int32
+    lib.nop_gated_forward.argtypes = [ctypes.POINTER(NopGatedDesc), ctypes.POINTER(NopGatedOperands), vp,
+                                      ctypes.c_size_t, vp]
+    lib.nop_gated_backward.restype = ctypes.c_int32
+    lib.nop_gated_backward.argtypes = [ctypes.POINTER(NopGatedDesc), ctypes.POINTER(NopGatedOperands),
+                                       ctypes.POINTER(NopGatedGrads), vp, ctypes.c_size_t, vp]
     lib.nop_clip_workspace_size.restype = ctypes.c_int32
     lib.nop_clip_workspace_size.argtypes = [ctypes.c_int32, size]
     lib.nop_clip_by_norm.restype = ctypes.c_int32

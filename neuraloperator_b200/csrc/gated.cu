@@ -1,0 +1,1513 @@
+// Gated feed-forward block at every point of a field, forward and backward, on the tensor cores (tcgen05).
+//
+//   g = W_gate x + b_gate,  u = W_up x + b_up,  h = act(g) u,  y = W_down h + b_down
+//
+// x [B, C, P], hidden width H, y [B, O, P]; act is SiLU or the exact GELU.  Backward, with e = dL/dy:
+//
+//   f = W_down^T e,  dg = f u act'(g),  du = f act(g),  dL/dx = W_gate^T dg + W_up^T du,
+//   dL/dW_gate = dg x^T,  dL/dW_up = du x^T,  dL/dW_down = e h^T (sums over all points), biases: row sums.
+//
+// Both passes are one kernel shape (k_block).  A tile is 128 points (the MMA's M); the hidden width is walked in
+// chunks of NH.  A job is one chunk of one tile:
+//   first product   D1 = [g | u] (backward: [g | u | f])   A = x (and e) from shared memory, B = weights
+//   middle          the epilogue warps read D1, apply the activation and write h (backward: dg, du) back into the
+//                   same columns of tensor memory as the next A operand -- h never leaves the SM in the forward
+//   second product  D2 += h W_down^T (backward: dg W_gate + du W_up), A from tensor memory
+// and after a tile's last chunk D2 goes out.  Two D1 buffers alternate, so the tensor core works on job k + 1's
+// first product while the epilogue warps work on job k; a tile's D2 is read after the next tile's first middle.
+//
+// Operands.  16-bit fields multiply as they are (products exact, fp32 sums).  fp32 values are split into three
+// bf16 parts, v = a + b + c to within 2^-26 |v|, and six of the nine products are summed (the three left out are
+// below 2^-26): fp32 accuracy at the cost of six 16-bit MMAs, the same tensor time as three tf32 passes on a
+// hi / lo split but three quarters of its shared memory, and 2^-26 instead of 2^-21.  The tensor core adds to its
+// accumulator with truncation, about 2^-25 of it towards zero every time, so the five smaller products, 2^-8 of the
+// first and less, are kept from the large accumulator: the second product gives them columns of their own (D2c,
+// added at the end), the first product adds them before the large one, piece by piece.  (All six into one
+// accumulator: dL/dx was 4.7e-6 off at 128 channels, hidden 200.)  An e4m3 field is widened exactly and its point's
+// scale multiplies the accumulator.
+//
+// The points of a channel are contiguous and the MMA wants a point's channels contiguous (K-major core matrices of
+// 8 rows x 16 bytes): a producer thread loads 8 channels x 4 points with one wide load a channel and writes four
+// 16-byte rows, so the transposition is a choice of registers.  The core matrices of 8-row groups lie 272 bytes
+// apart instead of 256: the rows that eight neighbouring threads write then fall into eight different 16-byte
+// columns of the banks.  Weights are packed once a call (k_pack) into images that a bulk copy brings into shared
+// memory whole; they stay there for the whole kernel when they fit, and stream through a ring otherwise.
+//
+// The weight gradients contract over points, which are contiguous in every operand: k_wgrad reads dg, du, h (left
+// by k_block in a scratch [3 H][points of a slab]), x and e, splits the points over the CTAs and leaves partial
+// sums that k_finish adds in a fixed order.  Because of the truncation a long sum is cut: every kPromote pieces the
+// epilogue warps add the accumulator (fp32: and the smaller products' own) to registers.
+// The scratch is made and consumed slab by slab, sized to stay in L2.
+//
+// Every wait is bounded: on expiry the kernel records NOP_DEVICE_MMA_TIMEOUT in the status word, all roles leave
+// their loops, copies and MMAs in flight are waited for (bounded) and the tensor memory is freed.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "mix_tc.cuh"
+
+namespace nop {
+namespace gated {
+
+constexpr int TP = 128;                       // points a tile
+constexpr int kEpi = 8;                       // warps 0..7: middle and output
+constexpr int kProd = 4;                      // warps 8..11: x (and e) into shared memory
+constexpr int kMma = kEpi + kProd;            // warp 12: MMA issue
+constexpr int kLoad = kMma + 1;               // warp 13: weight copies
+constexpr int kThreads = 32 * (kLoad + 1);
+constexpr int kSmem = 227 * 1024;
+constexpr int kAGroup = 272;                  // bytes between 8-row groups of an A image
+constexpr int kMaxA = 8, kMaxB = 8;           // ring slots at most
+
+__host__ __device__ constexpr int up16(int v) { return (v + 15) & ~15; }
+__host__ __device__ constexpr int imin(int a, int b) { return a < b ? a : b; }
+
+// Operand form of a field type: images an operand has, elements of K a ring piece has
+template <class T> struct Form {
+    static constexpr int SPL = 1, KC = 64;
+    static constexpr uint32_t kFmt = 1;       // bf16
+};
+template <> struct Form<float> {
+    static constexpr int SPL = 3, KC = 32;
+    static constexpr uint32_t kFmt = 1;
+};
+template <> struct Form<__half> {
+    static constexpr int SPL = 1, KC = 64;
+    static constexpr uint32_t kFmt = 0;
+};
+// the products of the images, largest first: (A image, B image)
+template <int SPL> struct Passes {
+    static constexpr int N = SPL == 1 ? 1 : 6;
+    __device__ static constexpr int a(int i) { return i == 2 || i == 3 ? 1 : i == 5 ? 2 : 0; }
+    __device__ static constexpr int b(int i) { return i == 1 || i == 3 ? 1 : i == 4 ? 2 : 0; }
+};
+
+struct Plan {
+    int C, H, O;               // channels of x, hidden width, channels of y
+    int Kx, Ky;                // padded K of the first products (Ky: backward only, 0 otherwise)
+    int cols, col0;            // channels of this launch's output, the first of them
+    int N2;                    // padded columns of D2
+    int NH, nJ;                // chunk width, chunks
+    int nKx, nKy, nH;          // ring pieces: of x, of e, of a chunk in the second product
+    int na, nb;                // ring slots (nb: streaming)
+    int reuse;                 // 1: a tile's A pieces stay in the ring for all its chunks
+    int resident;              // 1: all weight images stay in shared memory
+    int a_slot, b_slot;        // bytes
+    int job_bytes;             // packed weight bytes of one chunk
+    int o_a, o_b, o_bar, smem;
+};
+
+struct Params {
+    const void* x;
+    const void* gy;            // backward: e
+    const float* scale;        // e4m3 x: one a point
+    const char* packed;
+    const float *bg, *bu, *b2; // fp32, padded with zeros (b2: the output's, forward)
+    void* out;                 // y, or dL/dx (may be NULL)
+    void* z;                   // backward: [3 H][zs] dg, du, h (may be NULL)
+    int64_t zs;
+    uint32_t P, points;        // a sample's points, all points
+    int tile0, tiles;          // tiles of this launch
+    int vec;                   // 4 points a load
+    Plan pl;
+};
+
+__host__ __device__ inline int piece_k(int K, int KC, int kc) { return imin(KC, K - kc * KC); }
+
+// ------------------------------------------------------------------------------------------------
+// device helpers
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t desc_of(uint32_t addr, int sbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ uint32_t idesc_of(uint32_t fmt, int N) {
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(TP >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    tc::mma_bf16(d, a, b, idesc, acc ? 1u : 0u);
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+        :
+        : "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u), "r"(0), "r"(0), "r"(0), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// the registers are operands, so no use of them moves above the wait
+__device__ __forceinline__ void wait_ld(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+                   "+f"(v[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(bytes)
+                 : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// two neighbouring K elements as one word of each image
+template <class T> __device__ __forceinline__ void images(float v0, float v1, uint32_t (&w)[Form<T>::SPL]);
+template <> __device__ __forceinline__ void images<__nv_bfloat16>(float v0, float v1, uint32_t (&w)[1]) {
+    w[0] = tc::pack_bf16(v0, v1);
+}
+template <> __device__ __forceinline__ void images<__half>(float v0, float v1, uint32_t (&w)[1]) {
+    const __half2 h = __floats2half2_rn(v0, v1);
+    w[0] = *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ void images<float>(float v0, float v1, uint32_t (&w)[3]) {
+    // v = a + b + c, each part the rounding of what is left (the differences are exact)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        w[i] = tc::pack_bf16(v0, v1);
+        v0 -= __uint_as_float(w[i] << 16);
+        v1 -= __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+
+// act(g) and act'(g).  SiLU: g s, s (1 + g (1 - s)), s = 1 / (1 + exp(-g)).  GELU: g P(g), P(g) + g p(g) with the
+// normal distribution function P from erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + q x), Abramowitz &
+// Stegun, Handbook of Mathematical Functions (1964), eq. 7.1.26 (|error| <= 1.5e-7); its exponential is also the
+// density's.
+constexpr float kLog2e = 1.4426950408889634f;
+template <bool GELU>
+__device__ __forceinline__ float activation(float g, float& slope) {
+    if (!GELU) {
+        const float s = __fdividef(1.f, 1.f + exp2f(-kLog2e * g));
+        slope = s * fmaf(g, 1.f - s, 1.f);
+        return g * s;
+    }
+    const float x = fabsf(g) * 0.70710678118654752f;
+    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    const float e = exp2f(-kLog2e * x * x);
+    float s = fmaf(t, 1.061405429f, -1.453152027f);
+    s = fmaf(t, s, 1.421413741f);
+    s = fmaf(t, s, -0.284496736f);
+    s = fmaf(t, s, 0.254829592f);
+    const float tail = 0.5f * s * t * e;          // P(-|g|)
+    const float cdf = g < 0.f ? tail : 1.f - tail;
+    slope = fmaf(g * 0.3989422804014327f, e, cdf);
+    return g * cdf;
+}
+
+// ------------------------------------------------------------------------------------------------
+// weights -> images
+// ------------------------------------------------------------------------------------------------
+// One thread packs 8 elements of K of one row of one piece.  Chunk j's pieces follow one another: the first
+// product's (rows: NH of W_gate, NH of W_up; K: channels of x), backward the f product's (rows: NH hidden; K:
+// channels of e, from W_down), then the second product's (forward: rows O, K hidden, from W_down; backward: rows C,
+// K hidden, from W_gate and then from W_up).
+template <class T, bool BWD>
+__global__ void __launch_bounds__(256)
+k_pack(Plan pl, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ wd, const T* __restrict__ bg,
+       const T* __restrict__ bu, const T* __restrict__ bd, char* __restrict__ packed, float* __restrict__ vec) {
+    constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC;
+    const int hid = pl.NH * pl.nJ;
+    const int stride = gridDim.x * blockDim.x, first = blockIdx.x * blockDim.x + threadIdx.x;
+    for (int i = first; i < 2 * hid + pl.N2; i += stride) {
+        const int k = i < hid ? i : i < 2 * hid ? i - hid : i - 2 * hid;
+        const T* b = i < hid ? bg : i < 2 * hid ? bu : bd;
+        const int n = i < 2 * hid ? pl.H : (BWD ? 0 : pl.cols);
+        vec[i] = b && k < n ? to_f(b[i < 2 * hid ? k : pl.col0 + k]) : 0.f;
+    }
+    const int r1 = 2 * pl.NH, c1 = r1 * (pl.Kx / 8), c2 = BWD ? pl.NH * (pl.Ky / 8) : 0;
+    const int c3 = pl.N2 * (pl.NH / 8), per = c1 + c2 + (BWD ? 2 : 1) * c3;
+    for (int i = first; i < per * pl.nJ; i += stride) {
+        const int j = i / per;
+        int c = i % per, off = j * pl.job_bytes;
+        int rows, K, part;
+        if (c < c1) {
+            part = 0;
+            rows = r1;
+            K = pl.Kx;
+        } else if (c < c1 + c2) {
+            part = 1;
+            off += c1 * 16 * SPL;
+            c -= c1;
+            rows = pl.NH;
+            K = pl.Ky;
+        } else {
+            off += (c1 + c2) * 16 * SPL;
+            c -= c1 + c2;
+            part = 2;
+            if (c >= c3) {
+                c -= c3;
+                off += c3 * 16 * SPL;
+                part = 3;
+            }
+            rows = pl.N2;
+            K = pl.NH;
+        }
+        const int row = c % rows, k8 = c / rows;            // neighbouring threads: neighbouring rows
+        const int kc = k8 / (KC / 8), ch = k8 % (KC / 8), pw = piece_k(K, KC, kc);
+        off += rows * kc * KC * 2 * SPL;                     // the pieces before this one are full
+        off += (ch >> 1) * (rows * 32) + (row >> 3) * 256 + (ch & 1) * 128 + (row & 7) * 16;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = k8 * 8 + e;
+            float w = 0.f;
+            if (part == 0) {
+                const int h = j * pl.NH + (row < pl.NH ? row : row - pl.NH);
+                if (h < pl.H && k < pl.C) w = to_f((row < pl.NH ? wg : wu)[(int64_t)h * pl.C + k]);
+            } else if (part == 1) {
+                const int h = j * pl.NH + row;
+                if (h < pl.H && k < pl.O) w = to_f(wd[(int64_t)k * pl.H + h]);
+            } else {
+                const int h = j * pl.NH + k;
+                if (!BWD) {
+                    if (h < pl.H && row < pl.cols) w = to_f(wd[(int64_t)(pl.col0 + row) * pl.H + h]);
+                } else if (h < pl.H && row < pl.cols) {
+                    w = to_f((part == 2 ? wg : wu)[(int64_t)h * pl.C + pl.col0 + row]);
+                }
+            }
+            v[e] = w;
+        }
+        uint32_t img[4][SPL];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) images<T>(v[2 * e], v[2 * e + 1], img[e]);
+#pragma unroll
+        for (int s = 0; s < SPL; ++s)
+            *reinterpret_cast<uint4*>(packed + off + s * rows * pw * 2) =
+                make_uint4(img[0][s], img[1][s], img[2][s], img[3][s]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// x / e -> A images
+// ------------------------------------------------------------------------------------------------
+// 8 channels x 4 points as loaded: 16-bit and fp32 fields two or four words a channel, e4m3 one
+template <class IN> struct Item {
+    static constexpr int W = (int)sizeof(IN);  // words a channel
+    uint32_t w[8 * W];
+};
+
+// lane's 4 points: 4 lane .. 4 lane + 3 of the tile (vec), or lane, lane + 32, ... (any alignment)
+template <class IN>
+__device__ __forceinline__ void load_item(Item<IN>& it, const IN* __restrict__ src, int C, int c0, uint32_t n0, int lane,
+                                          const Params& p) {
+    constexpr int W = Item<IN>::W;
+    if (p.vec) {
+        const uint32_t n = n0 + 4 * lane;
+        const bool ok = n < p.points;
+        const uint32_t b = ok ? n / p.P : 0;
+        const IN* s = src + (int64_t)b * C * p.P + (ok ? n - b * p.P : 0) + (int64_t)c0 * p.P;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool in = ok && c0 + e < C;
+            const IN* a = s + (int64_t)e * p.P;
+            if constexpr (W == 4) {
+                const uint4 q = in ? __ldg(reinterpret_cast<const uint4*>(a)) : make_uint4(0, 0, 0, 0);
+                it.w[4 * e] = q.x;
+                it.w[4 * e + 1] = q.y;
+                it.w[4 * e + 2] = q.z;
+                it.w[4 * e + 3] = q.w;
+            } else if constexpr (W == 2) {
+                const uint2 q = in ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
+                it.w[2 * e] = q.x;
+                it.w[2 * e + 1] = q.y;
+            } else {
+                it.w[e] = in ? __ldg(reinterpret_cast<const uint32_t*>(a)) : 0;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8 * W; ++e) it.w[e] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t n = n0 + lane + 32 * i;
+        if (n >= p.points) continue;
+        const uint32_t b = n / p.P;
+        const IN* s = src + (int64_t)b * C * p.P + (n - b * p.P) + (int64_t)c0 * p.P;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (c0 + e >= C) continue;
+            const IN* a = s + (int64_t)e * p.P;
+            if constexpr (W == 4) it.w[4 * e + i] = __ldg(reinterpret_cast<const uint32_t*>(a));
+            else if constexpr (W == 2)
+                it.w[2 * e + i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(a)) << (16 * (i & 1));
+            else
+                it.w[e] |= (uint32_t)__ldg(reinterpret_cast<const uint8_t*>(a)) << (8 * i);
+        }
+    }
+}
+
+// the four points' rows of one 16-byte column (8 channels) of an A piece
+template <class T, class IN>
+__device__ __forceinline__ void store_item(const Item<IN>& it, char* slot, int ch, int steps, int lane, bool vec) {
+    constexpr int SPL = Form<T>::SPL;
+    char* base = slot + (ch >> 1) * (16 * kAGroup) + (ch & 1) * 128;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = vec ? 4 * lane + i : lane + 32 * i;
+        uint32_t img[4][SPL];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(IN) == 4) {
+                images<T>(__uint_as_float(it.w[8 * e + i]), __uint_as_float(it.w[8 * e + 4 + i]), img[e]);
+            } else if constexpr (sizeof(IN) == 2) {
+                img[e][0] = __byte_perm(it.w[4 * e + i / 2], it.w[4 * e + 2 + i / 2], i & 1 ? 0x7632 : 0x5410);
+            } else {
+                const uint32_t two = __byte_perm(it.w[2 * e], it.w[2 * e + 1], (uint32_t)(i | (4 + i) << 4));
+                const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffff), __NV_E4M3);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                images<T>(f.x, f.y, img[e]);  // exact
+            }
+        }
+        char* at = base + (row >> 3) * kAGroup + (row & 7) * 16;
+#pragma unroll
+        for (int s = 0; s < SPL; ++s)
+            *reinterpret_cast<uint4*>(at + s * steps * (16 * kAGroup)) =
+                make_uint4(img[0][s], img[1][s], img[2][s], img[3][s]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// the block kernel
+// ------------------------------------------------------------------------------------------------
+// barriers, by index into the barrier area
+struct Bars {
+    uint64_t full_a[kMaxA], empty_a[kMaxA], full_b[kMaxB], empty_b[kMaxB];
+    uint64_t d1[2], mid[2], g2[2], d2, d2_free, drain;
+    uint32_t tmem;
+    int abort_flag;
+};
+
+template <class T, class IN, bool BWD, bool GELU>
+__global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ Params p, int* __restrict__ status) {
+    constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N;
+    extern __shared__ __align__(1024) char sm[];
+    const Plan& pl = p.pl;
+    Bars& bar = *reinterpret_cast<Bars*>(sm + pl.o_bar);
+    volatile int* abort_flag = &bar.abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < kMaxA; ++i) {
+            tc::mbar_init(&bar.full_a[i], kProd);
+            tc::mbar_init(&bar.empty_a[i], 1);
+        }
+        for (int i = 0; i < kMaxB; ++i) {
+            tc::mbar_init(&bar.full_b[i], 1);
+            tc::mbar_init(&bar.empty_b[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&bar.d1[i], 1);
+            tc::mbar_init(&bar.mid[i], kEpi);
+            tc::mbar_init(&bar.g2[i], 1);
+        }
+        tc::mbar_init(&bar.d2, 1);
+        tc::mbar_init(&bar.d2_free, kEpi);
+        tc::mbar_init(&bar.drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        bar.abort_flag = 0;
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc::smem_u32(&bar.tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = bar.tmem;
+    auto give_up = [&]() {
+        *abort_flag = 1;
+        atomicExch(status, tc::kStatusMmaTimeout);
+    };
+    auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
+        if (tc::mbar_wait(b, parity, abort_flag)) return true;
+        give_up();
+        return false;
+    };
+
+    const int my = p.tiles > (int)blockIdx.x ? (p.tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    const int jobs = my * pl.nJ;
+    const int nA = pl.nKx + pl.nKy;                       // A pieces of a job
+    const int d1w = (BWD ? 3 : 2) * pl.NH;                // columns of a D1 buffer
+    const uint32_t d2 = tmem + 2 * d1w;
+    auto tile_at = [&](int k) { return (uint32_t)(p.tile0 + (int)blockIdx.x + k * (int)gridDim.x); };
+
+    if (warp >= kEpi && warp < kMma) {
+        // ------------------------------ x / e -> shared memory ------------------------------
+        // a warp takes the 16-byte columns w, w + 4 of every piece; x and e have the same type in the backward
+        const int w = warp - kEpi;
+        constexpr int NI = KC / 32;                       // items a thread has in a piece
+        const int total = (pl.reuse ? my : jobs) * nA;
+        auto load = [&](Item<IN>(&it)[NI], int a) {
+            const int kc = a % nA;
+            const uint32_t n0 = tile_at(a / nA / (pl.reuse ? 1 : pl.nJ)) * TP;
+            const bool is_x = !BWD || kc < pl.nKx;
+            const IN* src = static_cast<const IN*>(is_x ? p.x : p.gy);
+            const int k0 = (is_x ? kc : kc - pl.nKx) * KC;
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                load_item<IN>(it[i], src, is_x ? pl.C : pl.O, k0 + (w + 4 * i) * 8, n0, lane, p);
+        };
+        auto put = [&](const Item<IN>(&it)[NI], int a) -> bool {
+            const int kc = a % nA, slot = a % pl.na, use = a / pl.na;
+            const int pw = !BWD || kc < pl.nKx ? piece_k(pl.Kx, KC, kc) : piece_k(pl.Ky, KC, kc - pl.nKx);
+            if (use > 0 && !wait(&bar.empty_a[slot], (uint32_t)(use - 1) & 1)) return false;
+            char* s = sm + pl.o_a + slot * pl.a_slot;
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                if ((w + 4 * i) * 8 < pw) store_item<T, IN>(it[i], s, w + 4 * i, pw / 16, lane, p.vec);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bar.full_a[slot]);
+            return true;
+        };
+        // the next piece's loads are in flight while this one waits for its slot and is written
+        Item<IN> c[NI], d[NI];
+        if (total > 0) load(c, 0);
+        for (int a = 0; a < total; a += 2) {
+            if (a + 1 < total) load(d, a + 1);
+            if (!put(c, a)) break;
+            if (a + 1 >= total) break;
+            if (a + 2 < total) load(c, a + 2);
+            if (!put(d, a + 1)) break;
+        }
+    } else if (warp == kLoad) {
+        // ------------------------------ weights -> shared memory ------------------------------
+        if (lane == 0 && jobs > 0) {
+            const uint32_t sb = tc::smem_u32(sm + pl.o_b);
+            if (pl.resident) {
+                bulk_copy(sb, p.packed, (uint32_t)(pl.nJ * pl.job_bytes), &bar.full_b[0]);
+                tc::mbar_wait(&bar.full_b[0], 0, nullptr);  // no copy outlives the CTA (bounded)
+            } else {
+                int q = 0;
+                bool ok = true;
+                auto push = [&](const char* src, int rows, int pw) -> int {
+                    const int slot = q % pl.nb, use = q / pl.nb, bytes = rows * pw * 2 * SPL;
+                    if (use > 0 && !wait(&bar.empty_b[slot], (uint32_t)(use - 1) & 1)) {
+                        ok = false;
+                        return 0;
+                    }
+                    bulk_copy(sb + slot * pl.b_slot, src, (uint32_t)bytes, &bar.full_b[slot]);
+                    ++q;
+                    return bytes;
+                };
+                for (int J = 0; J <= jobs && ok; ++J) {  // in the order of the MMA warp
+                    if (J < jobs) {
+                        const char* src = p.packed + (int64_t)(J % pl.nJ) * pl.job_bytes;
+                        for (int kc = 0; kc < pl.nKx && ok; ++kc) src += push(src, 2 * pl.NH, piece_k(pl.Kx, KC, kc));
+                        for (int kc = 0; kc < pl.nKy && ok; ++kc) src += push(src, pl.NH, piece_k(pl.Ky, KC, kc));
+                    }
+                    if (J > 0 && ok) {
+                        const char* src = p.packed + (int64_t)((J - 1) % pl.nJ) * pl.job_bytes +
+                                          (int64_t)pl.NH * (2 * pl.Kx + pl.Ky) * 2 * SPL;
+                        for (int m = 0; m < (BWD ? 2 : 1); ++m)
+                            for (int kc = 0; kc < pl.nH && ok; ++kc) src += push(src, pl.N2, piece_k(pl.NH, KC, kc));
+                    }
+                }
+                for (int i = 0; i < pl.nb && i < q; ++i) {  // no copy outlives the CTA (bounded)
+                    const int last = q - 1 - i;
+                    tc::mbar_wait(&bar.full_b[last % pl.nb], (uint32_t)(last / pl.nb) & 1, nullptr);
+                }
+            }
+        }
+    } else if (warp == kMma) {
+        // ------------------------------ MMA issue ------------------------------
+        if (lane == 0 && jobs > 0) {
+            const uint32_t sa = tc::smem_u32(sm + pl.o_a), sb = tc::smem_u32(sm + pl.o_b);
+            constexpr uint32_t fmt = Form<T>::kFmt;
+            int q = 0;
+            bool ok = !pl.resident || wait(&bar.full_b[0], 0);
+            // the images of the next weight piece (`at`: its place among its chunk's, when resident)
+            auto weights = [&](int j, int at) -> uint32_t {
+                if (pl.resident) return sb + (uint32_t)(j * pl.job_bytes + at);
+                if (!wait(&bar.full_b[q % pl.nb], (uint32_t)(q / pl.nb) & 1)) ok = false;
+                return sb + (uint32_t)((q % pl.nb) * pl.b_slot);
+            };
+            auto weights_done = [&]() {
+                if (pl.resident) return;
+                tc::mma_commit(&bar.empty_b[q % pl.nb]);
+                ++q;
+            };
+            // D (columns d ..) (+)= A piece from shared memory x B piece of N rows
+            auto product_ss = [&](uint32_t d, uint32_t a0, uint32_t b0, int N, int pw, bool acc) {
+                const int steps = pw / 16;
+                const uint32_t id = idesc_of(fmt, N);
+                uint64_t da[SPL], db[SPL];
+#pragma unroll
+                for (int s = 0; s < SPL; ++s) {
+                    da[s] = desc_of(a0 + s * steps * (16 * kAGroup), kAGroup);
+                    db[s] = desc_of(b0 + s * N * pw * 2, 256);
+                }
+                for (int ks = 0; ks < steps; ++ks) {  // the smaller products
+#pragma unroll
+                    for (int i = 1; i < NP; ++i) {
+                        mma_ss(d, da[Passes<SPL>::a(i)] + ks * (kAGroup), db[Passes<SPL>::b(i)] + ks * (N * 2), id, acc);
+                        acc = true;
+                    }
+                }
+                for (int ks = 0; ks < steps; ++ks) {
+                    mma_ss(d, da[0] + ks * kAGroup, db[0] + ks * (N * 2), id, acc);
+                    acc = true;
+                }
+            };
+            // ... x A images in tensor memory; image s of the K step of hidden group g at column col[s] + 16 g; the
+            // smaller products in the N columns after D's
+            auto product_ts = [&](uint32_t d, const uint32_t (&col)[SPL], uint32_t b0, int N, int pw, bool acc, int g0) {
+                const uint32_t id = idesc_of(fmt, N);
+                uint64_t db[SPL];
+#pragma unroll
+                for (int s = 0; s < SPL; ++s) db[s] = desc_of(b0 + s * N * pw * 2, 256);
+                for (int ks = 0; ks < pw / 16; ++ks) {
+#pragma unroll
+                    for (int i = 0; i < NP; ++i)
+                        mma_ts(i ? d + N : d, col[Passes<SPL>::a(i)] + 16 * (g0 + ks), db[Passes<SPL>::b(i)] + ks * (N * 2),
+                               id, i > 1 || acc);
+                    acc = true;
+                }
+            };
+            for (int J = 0; J <= jobs && ok; ++J) {
+                if (J < jobs) {  // first product of job J
+                    const int b = J & 1, j = J % pl.nJ, k = J / pl.nJ;
+                    if (J >= 2 && !wait(&bar.g2[b], (uint32_t)((J >> 1) - 1) & 1)) break;
+                    fence_after();
+                    const uint32_t d = tmem + b * d1w;
+                    int at = 0;
+                    for (int kc = 0; kc < nA && ok; ++kc) {
+                        const bool is_x = kc < pl.nKx;
+                        const int a = (pl.reuse ? k : J) * nA + kc, slot = a % pl.na;
+                        const int pw = is_x ? piece_k(pl.Kx, KC, kc) : piece_k(pl.Ky, KC, kc - pl.nKx);
+                        const int N = is_x ? 2 * pl.NH : pl.NH;
+                        if (!wait(&bar.full_a[slot], (uint32_t)(a / pl.na) & 1)) ok = false;
+                        const uint32_t wb = weights(j, at);
+                        if (!ok) break;
+                        fence_after();
+                        product_ss(is_x ? d : d + 2 * pl.NH, sa + slot * pl.a_slot, wb, N, pw, kc != 0 && kc != pl.nKx);
+                        at += N * pw * 2 * SPL;
+                        weights_done();
+                        if (!pl.reuse || j == pl.nJ - 1) tc::mma_commit(&bar.empty_a[slot]);
+                    }
+                    if (!ok) break;
+                    tc::mma_commit(&bar.d1[b]);
+                }
+                if (J > 0) {  // second product of job J - 1
+                    const int q1 = J - 1, b = q1 & 1, j = q1 % pl.nJ, k = q1 / pl.nJ;
+                    if (!wait(&bar.mid[b], (uint32_t)(q1 >> 1) & 1)) break;
+                    if (j == 0 && k > 0 && !wait(&bar.d2_free, (uint32_t)(k - 1) & 1)) break;
+                    fence_after();
+                    const uint32_t d = tmem + b * d1w;
+                    int at = pl.NH * (2 * pl.Kx + pl.Ky) * 2 * SPL;
+                    for (int m = 0; m < (BWD ? 2 : 1); ++m) {
+                        uint32_t col[SPL];  // the places that the middle gave the images (k_block's epilogue)
+                        if constexpr (SPL == 1) {
+                            col[0] = d + m * pl.NH;
+                        } else {
+                            col[0] = m ? d + pl.NH + 8 : d;
+                            col[1] = m ? d + 2 * pl.NH : d + 8;
+                            col[2] = m ? d + 2 * pl.NH + 8 : d + pl.NH;
+                        }
+                        for (int kc = 0; kc < pl.nH; ++kc) {
+                            const int pw = piece_k(pl.NH, KC, kc);
+                            const uint32_t wb = weights(j, at);
+                            if (!ok) break;
+                            fence_after();
+                            product_ts(d2, col, wb, pl.N2, pw, j != 0 || m != 0 || kc != 0, kc * (KC / 16));
+                            at += pl.N2 * pw * 2 * SPL;
+                            weights_done();
+                        }
+                        if (!ok) break;
+                    }
+                    if (!ok) break;
+                    tc::mma_commit(&bar.g2[b]);
+                    if (j == pl.nJ - 1) tc::mma_commit(&bar.d2);
+                }
+            }
+            // every MMA issued has completed before the tensor memory is freed (bounded)
+            tc::mma_commit(&bar.drain);
+            tc::mbar_wait(&bar.drain, 0, nullptr);
+        }
+    } else if (warp < kEpi) {
+        // ------------------------------ middle and output ------------------------------
+        const int quad = warp & 3, half = warp >> 2;      // lane quadrant; which 16-column groups
+        const int row = quad * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const int groups = pl.NH / 16;
+
+        auto middle = [&](int J) -> bool {
+            const int b = J & 1, j = J % pl.nJ;
+            const uint32_t tile = tile_at(J / pl.nJ), n = tile * TP + row;
+            const bool valid = n < p.points;
+            float sc = 1.f;
+            if constexpr (sizeof(IN) == 1) sc = valid ? __ldg(p.scale + n) : 0.f;
+            if (!wait(&bar.d1[b], (uint32_t)(J >> 1) & 1)) return false;
+            fence_after();
+            const uint32_t d = tmem + b * d1w + lanes;
+            for (int g = half; g < groups; g += 2) {
+                float vg[16], vu[16];
+                ld16(d + 16 * g, vg);
+                ld16(d + pl.NH + 16 * g, vu);
+                wait_ld(vg);
+                wait_ld(vu);
+                const int h0 = j * pl.NH + 16 * g;
+                const float4* bg = reinterpret_cast<const float4*>(p.bg + h0);
+                const float4* bu = reinterpret_cast<const float4*>(p.bu + h0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 a = __ldg(bg + i), c = __ldg(bu + i);
+                    vg[4 * i] = fmaf(vg[4 * i], sc, a.x);
+                    vg[4 * i + 1] = fmaf(vg[4 * i + 1], sc, a.y);
+                    vg[4 * i + 2] = fmaf(vg[4 * i + 2], sc, a.z);
+                    vg[4 * i + 3] = fmaf(vg[4 * i + 3], sc, a.w);
+                    vu[4 * i] = fmaf(vu[4 * i], sc, c.x);
+                    vu[4 * i + 1] = fmaf(vu[4 * i + 1], sc, c.y);
+                    vu[4 * i + 2] = fmaf(vu[4 * i + 2], sc, c.z);
+                    vu[4 * i + 3] = fmaf(vu[4 * i + 3], sc, c.w);
+                }
+                if constexpr (!BWD) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float slope;
+                        vg[i] = activation<GELU>(vg[i], slope) * vu[i];
+                    }
+                    uint32_t w[SPL][8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t t[SPL];
+                        images<T>(vg[2 * i], vg[2 * i + 1], t);
+#pragma unroll
+                        for (int s = 0; s < SPL; ++s) w[s][i] = t[s];
+                    }
+                    st8(d + 16 * g, w[0]);
+                    if constexpr (SPL == 3) {
+                        st8(d + 16 * g + 8, w[1]);
+                        st8(d + pl.NH + 16 * g, w[2]);
+                    }
+                } else {
+                    float vf[16];
+                    ld16(d + 2 * pl.NH + 16 * g, vf);
+                    wait_ld(vf);
+                    T* z = static_cast<T*>(p.z) + (int64_t)h0 * p.zs + (int64_t)(tile - p.tile0) * TP + row;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float slope;
+                        const float a = activation<GELU>(vg[i], slope);
+                        const float h = a * vu[i];
+                        // points past the last one hold a product of zeros: their rows of the scratch are zeros
+                        vg[i] = valid ? vf[i] * vu[i] * slope : 0.f;
+                        vu[i] = valid ? vf[i] * a : 0.f;
+                        if (p.z && h0 + i < pl.H) {
+                            z[(int64_t)i * p.zs] = from_f<T>(vg[i]);
+                            z[(int64_t)(pl.H + i) * p.zs] = from_f<T>(vu[i]);
+                            z[(int64_t)(2 * pl.H + i) * p.zs] = from_f<T>(valid ? h : 0.f);
+                        }
+                    }
+                    uint32_t w[2][SPL][8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t t[SPL], r[SPL];
+                        images<T>(vg[2 * i], vg[2 * i + 1], t);
+                        images<T>(vu[2 * i], vu[2 * i + 1], r);
+#pragma unroll
+                        for (int s = 0; s < SPL; ++s) {
+                            w[0][s][i] = t[s];
+                            w[1][s][i] = r[s];
+                        }
+                    }
+                    if constexpr (SPL == 1) {
+                        st8(d + 16 * g, w[0][0]);
+                        st8(d + pl.NH + 16 * g, w[1][0]);
+                    } else {
+                        st8(d + 16 * g, w[0][0]);
+                        st8(d + 16 * g + 8, w[0][1]);
+                        st8(d + pl.NH + 16 * g, w[0][2]);
+                        st8(d + pl.NH + 16 * g + 8, w[1][0]);
+                        st8(d + 2 * pl.NH + 16 * g, w[1][1]);
+                        st8(d + 2 * pl.NH + 16 * g + 8, w[1][2]);
+                    }
+                }
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bar.mid[b]);
+            return true;
+        };
+        auto output = [&](int k) -> bool {
+            const uint32_t n = tile_at(k) * TP + row;
+            const bool valid = n < p.points;
+            const int width = BWD ? pl.C : pl.O;      // the field's channels
+            const uint32_t b = valid ? n / p.P : 0;
+            T* y = static_cast<T*>(p.out) + ((int64_t)b * width + pl.col0) * p.P + (valid ? n - b * p.P : 0);
+            if (!wait(&bar.d2, (uint32_t)k & 1)) return false;
+            fence_after();
+            for (int g = half; g < pl.N2 / 16; g += 2) {
+                float v[16];
+                ld16(d2 + lanes + 16 * g, v);
+                wait_ld(v);
+                if constexpr (SPL == 3) {
+                    float c[16];
+                    ld16(d2 + pl.N2 + lanes + 16 * g, c);
+                    wait_ld(c);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] += c[i];
+                }
+                if (!valid || !p.out) continue;
+                T* yg = y + (int64_t)(16 * g) * p.P;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (!BWD) v[i] += __ldg(p.b2 + 16 * g + i);
+                    if (16 * g + i < pl.cols) yg[(int64_t)i * p.P] = from_f<T>(v[i]);
+                }
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bar.d2_free);
+            return true;
+        };
+        bool ok = true;
+        for (int J = 0; J < jobs && ok; ++J) {
+            ok = middle(J);
+            if (ok && J > 0 && J % pl.nJ == 0) ok = output(J / pl.nJ - 1);
+        }
+        if (ok && my > 0) output(my - 1);
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// ------------------------------------------------------------------------------------------------
+// weight gradients
+// ------------------------------------------------------------------------------------------------
+constexpr int kWThreads = 32 * 16;            // warps 0..7 epilogue (warp 0 also issues the MMAs), 8..15 producers
+constexpr int kPromote = 8;                   // pieces an accumulator runs before it goes to registers
+constexpr int kWStages = 3;
+
+struct WParams {
+    const void *z, *x, *gy;
+    int64_t zs;
+    float* partial;            // [split][tile][128][128]
+    double* sums;              // [split][2 H + O] row sums of dg, du and e
+    int C, H, O;
+    uint32_t P, points;        // a sample's points, all points
+    uint32_t first;            // the slab's first point
+    int pieces;                // pieces of KC points in the slab
+    int splits;
+    int nC, nO;                // column tiles of x and of e
+    int mX, mH;                // row tiles of [dg; du] and of h
+    int accumulate;            // add to the partial sums of the slabs before
+    int vec;                   // 8 points of x and e a wide load
+};
+
+struct WBars {
+    uint64_t full[kWStages], empty[kWStages], acc[2], acc_free[2], drain;
+    uint32_t tmem;
+    int abort_flag;
+};
+
+// 8 points of one row
+template <class T> struct Eight {
+    static constexpr int W = (int)sizeof(T) * 2;
+    uint32_t w[W];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load_wide(const T* a) {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(a) + i);
+            w[4 * i] = q.x;
+            w[4 * i + 1] = q.y;
+            w[4 * i + 2] = q.z;
+            w[4 * i + 3] = q.w;
+        }
+    }
+    __device__ __forceinline__ void put(int i, const T* a) {
+        if constexpr (sizeof(T) == 4) w[i] = __ldg(reinterpret_cast<const uint32_t*>(a));
+        else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(a)) << (16 * (i & 1));
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else {
+            const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+            return to_f(*reinterpret_cast<const T*>(&h));
+        }
+    }
+};
+
+template <class T>
+__device__ __forceinline__ void store_eight(const Eight<T>& v, char* at, int image_bytes) {
+    constexpr int SPL = Form<T>::SPL;
+    if constexpr (SPL == 1) {
+        *reinterpret_cast<uint4*>(at) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    } else {
+        uint32_t img[4][SPL];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) images<T>(v.get(2 * e), v.get(2 * e + 1), img[e]);
+#pragma unroll
+        for (int s = 0; s < SPL; ++s)
+            *reinterpret_cast<uint4*>(at + s * image_bytes) = make_uint4(img[0][s], img[1][s], img[2][s], img[3][s]);
+    }
+}
+
+// CTA = (tile, split).  Tile: 128 rows of the scratch (rows of [dg; du] against channels of x, rows of h against
+// channels of e) x 128 channels; K: the split's share of the slab's points.
+template <class T>
+__global__ void __launch_bounds__(kWThreads, 1) k_wgrad(const __grid_constant__ WParams p, int* __restrict__ status) {
+    constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N;
+    constexpr int IMG = 128 * KC * 2, SLOT = 2 * SPL * IMG;   // A images, then B images
+    constexpr int DW = SPL == 3 ? 256 : 128;                  // columns of an accumulator (and the smaller products')
+    extern __shared__ __align__(1024) char sm[];
+    WBars& bar = *reinterpret_cast<WBars*>(sm + kWStages * SLOT);
+    volatile int* abort_flag = &bar.abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < kWStages; ++i) {
+            tc::mbar_init(&bar.full[i], 8);
+            tc::mbar_init(&bar.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&bar.acc[i], 1);
+            tc::mbar_init(&bar.acc_free[i], 8);
+        }
+        tc::mbar_init(&bar.drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        bar.abort_flag = 0;
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&bar.tmem)),
+                     "n"(2 * DW)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = bar.tmem;
+    auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
+        if (tc::mbar_wait(b, parity, abort_flag)) return true;
+        *abort_flag = 1;
+        atomicExch(status, tc::kStatusMmaTimeout);
+        return false;
+    };
+    const int tiles = p.mX * p.nC + p.mH * p.nO;
+    const int tile = (int)blockIdx.x % tiles, split = (int)blockIdx.x / tiles;
+    const bool of_x = tile < p.mX * p.nC;
+    const int mt = of_x ? tile / p.nC : (tile - p.mX * p.nC) / p.nO, nt = of_x ? tile % p.nC : (tile - p.mX * p.nC) % p.nO;
+    const int a_rows = of_x ? 2 * p.H - mt * 128 : p.H - mt * 128;     // rows left from the tile's first
+    const int b_rows = of_x ? p.C - nt * 128 : p.O - nt * 128;
+    const int n = imin(128, up16(b_rows));
+    const int k0 = (int)((int64_t)p.pieces * split / p.splits), k1 = (int)((int64_t)p.pieces * (split + 1) / p.splits);
+    const int steps = k1 - k0, runs = (steps + kPromote - 1) / kPromote;
+
+    if (warp >= 8 && warp < 16) {
+        // ------------------------------ producers ------------------------------
+        // lane: row lane % 8 of an 8-row group, 16-byte column lane / 8 (+ 4); warp w: groups w and w + 8
+        constexpr int NI = KC / 32;
+        const int w = warp - 8, r8 = lane & 7, ch0 = lane >> 3;
+        const int bc = of_x ? p.C : p.O;
+        const T* za = static_cast<const T*>(p.z) + (int64_t)((of_x ? 0 : 2 * p.H) + mt * 128) * p.zs;
+        const T* xb = static_cast<const T*>(of_x ? p.x : p.gy) + (int64_t)nt * 128 * p.P;
+        double sum_a[2] = {0.0, 0.0}, sum_b[2] = {0.0, 0.0};
+        const bool want_a = p.sums && of_x && nt == 0, want_b = p.sums && !of_x && mt == 0;
+        Eight<T> ca[2][NI], cb[2][NI], na[2][NI], nb[2][NI];
+        auto load = [&](Eight<T>(&ia)[2][NI], Eight<T>(&ib)[2][NI], int k) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const uint32_t q = (uint32_t)(k0 + k) * KC + (ch0 + 4 * i) * 8;  // point within the slab
+                const uint32_t pt = p.first + q;
+                const uint32_t b = pt < p.points ? pt / p.P : 0, o = pt < p.points ? pt - b * p.P : 0;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int r = (w + 8 * g) * 8 + r8;
+                    if (r < a_rows) ia[g][i].load_wide(za + (int64_t)r * p.zs + q);
+                    else ia[g][i].zero();
+                    if (r >= b_rows || pt >= p.points) {
+                        ib[g][i].zero();
+                    } else if (p.vec) {
+                        ib[g][i].load_wide(xb + ((int64_t)b * bc + r) * p.P + o);
+                    } else {
+                        ib[g][i].zero();
+                        uint32_t bb = b, oo = o;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (pt + e < p.points) ib[g][i].put(e, xb + ((int64_t)bb * bc + r) * p.P + oo);
+                            if (++oo == p.P) {
+                                oo = 0;
+                                ++bb;
+                            }
+                        }
+                    }
+                }
+            }
+        };
+        auto put = [&](const Eight<T>(&ia)[2][NI], const Eight<T>(&ib)[2][NI], int k) -> bool {
+            const int slot = k % kWStages, use = k / kWStages;
+            if (use > 0 && !wait(&bar.empty[slot], (uint32_t)(use - 1) & 1)) return false;
+            char* s = sm + slot * SLOT;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                float ta = 0.f, tb = 0.f;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const int ch = ch0 + 4 * i, off = (ch >> 1) * (128 * 32) + (w + 8 * g) * 256 + (ch & 1) * 128 + r8 * 16;
+                    store_eight<T>(ia[g][i], s + off, IMG);
+                    if ((w + 8 * g) * 8 < n) store_eight<T>(ib[g][i], s + SPL * IMG + off, IMG);
+                    if (want_a) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) ta += ia[g][i].get(e);
+                    }
+                    if (want_b) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) tb += ib[g][i].get(e);
+                    }
+                }
+                sum_a[g] += (double)ta;
+                sum_b[g] += (double)tb;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bar.full[slot]);
+            return true;
+        };
+        if (steps > 0) load(ca, cb, 0);
+        for (int k = 0; k < steps; k += 2) {
+            if (k + 1 < steps) load(na, nb, k + 1);
+            if (!put(ca, cb, k)) break;
+            if (k + 1 >= steps) break;
+            if (k + 2 < steps) load(ca, cb, k + 2);
+            if (!put(na, nb, k + 1)) break;
+        }
+        if (want_a || want_b) {
+            double* out = p.sums + (int64_t)split * (2 * p.H + p.O) + (want_a ? mt * 128 : 2 * p.H + nt * 128);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                double v = want_a ? sum_a[g] : sum_b[g];
+                v += __shfl_xor_sync(0xffffffffu, v, 8);
+                v += __shfl_xor_sync(0xffffffffu, v, 16);
+                const int r = (w + 8 * g) * 8 + r8;
+                if (lane < 8 && r < (want_a ? a_rows : b_rows)) out[r] = p.accumulate ? out[r] + v : v;
+            }
+        }
+    } else if (warp < 8) {
+        // ------------------------------ accumulators -> registers -> partial sums ------------------------------
+        const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+        float sum[4][16];   // groups of 16 columns half, half + 2, ...
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[g][i] = 0.f;
+        // run r's MMAs (kPromote pieces into accumulator r & 1), by warp 0's first lane
+        const uint32_t s0 = tc::smem_u32(sm);
+        const uint32_t id = idesc_of(Form<T>::kFmt, n);
+        auto issue = [&](int r) {
+            const int buf = r & 1;
+            if (r >= 2 && !wait(&bar.acc_free[buf], (uint32_t)((r >> 1) - 1) & 1)) return;
+            fence_after();
+            bool acc = false;
+            for (int k = r * kPromote; k < imin(steps, (r + 1) * kPromote); ++k) {
+                const int slot = k % kWStages;
+                if (!wait(&bar.full[slot], (uint32_t)(k / kWStages) & 1)) return;
+                fence_after();
+                const uint32_t a0 = s0 + slot * SLOT, b0 = a0 + SPL * IMG;
+#pragma unroll
+                for (int ks = 0; ks < KC / 16; ++ks) {
+#pragma unroll
+                    for (int i = 0; i < NP; ++i)
+                        mma_ss(tmem + buf * DW + (i ? 128 : 0), desc_of(a0 + Passes<SPL>::a(i) * IMG + ks * 128 * 32, 256),
+                               desc_of(b0 + Passes<SPL>::b(i) * IMG + ks * 128 * 32, 256), id, i > 1 || acc);
+                    acc = true;
+                }
+                tc::mma_commit(&bar.empty[slot]);
+            }
+            tc::mma_commit(&bar.acc[buf]);
+        };
+        const bool issuer = tid == 0;
+        if (issuer && runs > 0) issue(0);
+        bool ok = true;
+        for (int r = 0; r < runs; ++r) {
+            const int buf = r & 1;
+            if (issuer && r + 1 < runs) issue(r + 1);  // the tensor core works on r + 1 while r is read
+            __syncwarp();
+            if (!wait(&bar.acc[buf], (uint32_t)(r >> 1) & 1)) {
+                ok = false;
+                break;
+            }
+            fence_after();
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if ((half + 2 * g) * 16 < n) {
+                    float v[16];
+                    const uint32_t at = tmem + buf * DW + (half + 2 * g) * 16 + ((uint32_t)(quad * 32) << 16);
+                    ld16(at, v);
+                    wait_ld(v);
+                    if constexpr (SPL == 3) {
+                        float c[16];
+                        ld16(at + 128, c);
+                        wait_ld(c);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] += c[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[g][i] += v[i];
+                }
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bar.acc_free[buf]);
+        }
+        if (issuer) {  // every MMA issued has completed before the tensor memory is freed (bounded)
+            tc::mma_commit(&bar.drain);
+            tc::mbar_wait(&bar.drain, 0, nullptr);
+        }
+        if (ok && row < a_rows) {
+            float* out = p.partial + ((int64_t)split * tiles + tile) * (128 * 128) + row * 128;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if ((half + 2 * g) * 16 >= n) continue;
+                float4* o4 = reinterpret_cast<float4*>(out + (half + 2 * g) * 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float4 v = make_float4(sum[g][4 * i], sum[g][4 * i + 1], sum[g][4 * i + 2], sum[g][4 * i + 3]);
+                    if (p.accumulate) {
+                        const float4 o = o4[i];
+                        v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+                    }
+                    o4[i] = v;
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * DW));
+}
+
+// the splits' partial sums added in 64 bits, in order
+template <class T>
+__global__ void __launch_bounds__(128)
+k_finish(WParams p, T* __restrict__ gwg, T* __restrict__ gwu, T* __restrict__ gwd, T* __restrict__ gbg,
+         T* __restrict__ gbu, T* __restrict__ gbd) {
+    const int tiles = p.mX * p.nC + p.mH * p.nO;
+    const int rows = 3 * p.H, r = blockIdx.x;
+    if (r < rows) {
+        const bool of_x = r < 2 * p.H;
+        const int q = of_x ? r : r - 2 * p.H, cols = of_x ? p.C : p.O;
+        for (int c = threadIdx.x; c < cols; c += 128) {
+            const int tile = of_x ? q / 128 * p.nC + c / 128 : p.mX * p.nC + q / 128 * p.nO + c / 128;
+            const float* src = p.partial + (int64_t)tile * (128 * 128) + q % 128 * 128 + c % 128;
+            double s = 0.0;
+            for (int k = 0; k < p.splits; ++k) s += (double)src[(int64_t)k * tiles * (128 * 128)];
+            if (r < p.H) {
+                if (gwg) gwg[(int64_t)r * p.C + c] = from_f<T>((float)s);
+            } else if (of_x) {
+                if (gwu) gwu[(int64_t)(r - p.H) * p.C + c] = from_f<T>((float)s);
+            } else if (gwd) {
+                gwd[(int64_t)c * p.H + q] = from_f<T>((float)s);
+            }
+        }
+        return;
+    }
+    const int all = 2 * p.H + p.O;
+    for (int c = (r - rows) * 128 + threadIdx.x; c < all; c += (gridDim.x - rows) * 128) {
+        T* out = c < p.H ? gbg : c < 2 * p.H ? gbu : gbd;
+        if (!out) continue;
+        double s = 0.0;
+        for (int k = 0; k < p.splits; ++k) s += p.sums[(int64_t)k * all + c];
+        out[c < p.H ? c : c < 2 * p.H ? c - p.H : c - 2 * p.H] = from_f<T>((float)s);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------------
+// How a call is cut.  An fp32 launch takes at most 128 output channels (D2 and D2c); more are several launches, each
+// with the whole first product.  Tensor memory: two D1 buffers and D2 (fp32: and D2c) in 512 columns, so the
+// backward's chunk (three columns a hidden channel) is 64 wide when D2 takes up to 128 of them and 32 above.  Shared memory: the weights stay when they
+// leave room for two pieces of A, otherwise two to four pieces of each stream.
+template <class T>
+bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
+    constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC;
+    Plan p{};
+    p.C = d.channels;
+    p.H = d.hidden;
+    p.O = d.out_channels;
+    p.Kx = up16(p.C);
+    p.Ky = bwd ? up16(p.O) : 0;
+    p.col0 = col0;
+    p.cols = imin((bwd ? p.C : p.O) - col0, SPL == 3 ? 128 : 256);
+    p.N2 = up16(p.cols);
+    const int most = bwd && p.N2 * (SPL == 3 ? 2 : 1) > 128 ? 32 : 64;
+    p.nJ = (p.H + most - 1) / most;
+    p.NH = up16((p.H + p.nJ - 1) / p.nJ);
+    p.nKx = (p.Kx + KC - 1) / KC;
+    p.nKy = (p.Ky + KC - 1) / KC;
+    p.nH = (p.NH + KC - 1) / KC;
+    const int kx = imin(KC, std::max(p.Kx, p.Ky)), kh = imin(KC, p.NH);
+    p.a_slot = (kx / 16) * 16 * kAGroup * SPL;
+    p.b_slot = std::max(2 * p.NH * imin(KC, p.Kx), std::max(p.NH * imin(KC, p.Ky), p.N2 * kh)) * 2 * SPL;
+    p.job_bytes = (p.NH * (2 * p.Kx + p.Ky) + (bwd ? 2 : 1) * p.N2 * p.NH) * 2 * SPL;
+    const int64_t room = kSmem - 1024 - (int64_t)sizeof(Bars);
+    const int64_t all = (int64_t)p.nJ * p.job_bytes;
+    const int nA = p.nKx + p.nKy;
+    int64_t bytes;
+    if (all + 2 * p.a_slot <= room) {
+        p.resident = 1;
+        p.nb = 1;
+        p.na = (int)std::min<int64_t>(kMaxA, (room - all) / p.a_slot);
+        bytes = all;
+    } else {
+        p.nb = 2;
+        if (2 * p.a_slot + 2 * (int64_t)p.b_slot > room) return false;
+        // spare room: first for as many A pieces as a tile has, then for weights
+        p.na = 2;
+        while (p.na < kMaxA && p.na < nA && (p.na + 1) * p.a_slot + 2 * (int64_t)p.b_slot <= room) ++p.na;
+        while (p.nb < 4 && p.na * p.a_slot + (p.nb + 1) * (int64_t)p.b_slot <= room) ++p.nb;
+        while (p.na < kMaxA && (p.na + 1) * p.a_slot + p.nb * (int64_t)p.b_slot <= room) ++p.na;
+        bytes = (int64_t)p.nb * p.b_slot;
+    }
+    p.reuse = p.nJ > 1 && p.na >= nA;
+    p.o_a = 0;
+    p.o_b = p.na * p.a_slot;
+    p.o_b = (p.o_b + 127) & ~127;
+    p.o_bar = (int)((p.o_b + bytes + 127) & ~127);
+    p.smem = std::max(p.o_bar + (int)sizeof(Bars), 120 * 1024);  // one CTA an SM: it holds the whole tensor memory
+    *out = p;
+    return p.smem <= kSmem;
+}
+
+constexpr const char* kTooLarge = "these channel counts do not fit a CTA's shared memory";
+
+struct Sizes {
+    size_t packed, vec, z, partial, sums, bytes;
+    int64_t slab_tiles, tiles;
+    int splits, wtiles;
+};
+
+template <class T>
+Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd) {
+    auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
+    Sizes s{};
+    s.tiles = ceil_div(d.batch * d.points, TP);
+    size_t at = 0, images = 0, vectors = 0;
+    for (Plan q = p;;) {  // the launches of a call use the same places in turn
+        images = std::max(images, (size_t)q.nJ * q.job_bytes);
+        vectors = std::max(vectors, (size_t)(2 * q.NH * q.nJ + q.N2) * 4);
+        if (q.col0 + q.cols >= (bwd ? q.C : q.O) || !make_plan<T>(d, bwd, q.col0 + q.cols, &q)) break;
+    }
+    s.packed = at;
+    at += up(images);
+    s.vec = at;
+    at += up(vectors);
+    if (bwd) {
+        // the scratch of a slab stays within half of L2, in whole waves of 148 tiles
+        const int64_t tile_bytes = (int64_t)3 * p.H * TP * sizeof(T);
+        const int64_t waves = std::max<int64_t>(1, (int64_t)(64 << 20) / (148 * tile_bytes));
+        s.slab_tiles = std::min<int64_t>(s.tiles, 148 * waves);
+        s.wtiles = (int)(ceil_div(2 * p.H, 128) * ceil_div(p.C, 128) + ceil_div(p.H, 128) * ceil_div(p.O, 128));
+        const int64_t pieces = s.slab_tiles * (TP / Form<T>::KC);
+        s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(148 / s.wtiles, pieces));
+        s.z = at;
+        at += up((size_t)s.slab_tiles * tile_bytes);
+        s.partial = at;
+        at += up((size_t)s.splits * s.wtiles * 128 * 128 * 4);
+        s.sums = at;
+        at += up((size_t)s.splits * (2 * p.H + p.O) * 8);
+    }
+    s.bytes = at;
+    return s;
+}
+
+int32_t check(const nop_gated_desc* d) {
+    if (!d) return fail(NOP_E_INVALID, "descriptor is NULL");
+    if (d->abi_version != NOP_ABI_VERSION) return fail(NOP_E_INVALID, "ABI version mismatch");
+    if (d->dtype < NOP_DTYPE_FP32 || d->dtype > NOP_DTYPE_FP16) return fail(NOP_E_INVALID, "unknown dtype");
+    if (d->x_dtype != d->dtype && d->x_dtype != NOP_DTYPE_E4M3)
+        return fail(NOP_E_INVALID, "x has the weights' type, or e4m3");
+    if (d->x_dtype == NOP_DTYPE_E4M3 && d->dtype == NOP_DTYPE_FP32)
+        return fail(NOP_E_UNSUPPORTED, "an e4m3 field needs bf16 or fp16 weights");
+    if (d->activation != NOP_ACT_SILU && d->activation != NOP_ACT_GELU) return fail(NOP_E_INVALID, "unknown activation");
+    if (d->batch < 0 || d->points < 0) return fail(NOP_E_INVALID, "batch and points must be >= 0");
+    if (d->channels < 1 || d->hidden < 1 || d->out_channels < 1)
+        return fail(NOP_E_INVALID, "channels, hidden and out_channels must be positive");
+    if (d->channels > 256 || d->out_channels > 256)
+        return fail(NOP_E_UNSUPPORTED, "more than 256 channels are not supported");
+    if (d->hidden > 16384) return fail(NOP_E_UNSUPPORTED, "a hidden width above 16384 is not supported");
+    if (d->points && d->batch > (int64_t)0x7fffff00LL / d->points)
+        return fail(NOP_E_UNSUPPORTED, "more than 2^31 points");
+    return NOP_OK;
+}
+
+template <class F>
+int32_t by_type(int dtype, F&& f) {
+    if (dtype == NOP_DTYPE_FP32) return f(float{});
+    if (dtype == NOP_DTYPE_BF16) return f(__nv_bfloat16{});
+    return f(__half{});
+}
+
+struct Device {
+    int sms = 148;
+    int* status = nullptr;
+};
+int32_t device(Device* d) {
+    int dev = 0;
+    NOP_CUDA_TRY(cudaGetDevice(&dev));
+    NOP_CUDA_TRY(cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, dev));
+    d->status = status_word(dev);
+    if (!d->status) return fail(NOP_E_CUDA, "status word of the tensor-core kernels is not available");
+    return NOP_OK;
+}
+
+template <class K, class... A>
+int32_t launch(K kernel, unsigned grid, int threads, int smem, cudaStream_t s, A... args) {
+    NOP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<grid, threads, smem, s>>>(args...);
+    NOP_CUDA_TRY(cudaGetLastError());
+    return NOP_OK;
+}
+
+bool aligned(std::initializer_list<const void*> ps, uintptr_t to) {
+    uintptr_t all = 0;
+    for (const void* p : ps) all |= (uintptr_t)p;
+    return all % to == 0;
+}
+
+template <class T, bool BWD>
+int32_t pack(const Plan& p, const nop_gated_operands& o, const Sizes& z, char* ws, cudaStream_t s) {
+    const int items = (int)(((int64_t)p.nJ * p.job_bytes) / (16 * Form<T>::SPL));
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(items, 256), 592);
+    k_pack<T, BWD><<<grid, 256, 0, s>>>(p, static_cast<const T*>(o.w_gate), static_cast<const T*>(o.w_up),
+                                        static_cast<const T*>(o.w_down), static_cast<const T*>(o.b_gate),
+                                        static_cast<const T*>(o.b_up), static_cast<const T*>(o.b_down),
+                                        ws + z.packed, reinterpret_cast<float*>(ws + z.vec));
+    NOP_CUDA_TRY(cudaGetLastError());
+    return NOP_OK;
+}
+
+template <class T>
+Params params_of(const nop_gated_desc& d, const Plan& p, const nop_gated_operands& o, const Sizes& z, char* ws) {
+    Params q{};
+    q.x = o.x;
+    q.scale = o.x_scale;
+    q.packed = ws + z.packed;
+    q.bg = reinterpret_cast<const float*>(ws + z.vec);
+    q.bu = q.bg + p.NH * p.nJ;
+    q.b2 = q.bu + p.NH * p.nJ;
+    q.P = (uint32_t)d.points;
+    q.points = (uint32_t)(d.batch * d.points);
+    q.tiles = (int)z.tiles;
+    q.pl = p;
+    return q;
+}
+
+template <class T, class IN>
+int32_t forward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, const Sizes& z, char* ws, cudaStream_t s) {
+    Device dev;
+    int32_t rc = device(&dev);
+    if (rc != NOP_OK) return rc;
+    const unsigned grid = (unsigned)std::min<int64_t>(z.tiles, dev.sms);
+    while (true) {
+        if ((rc = pack<T, false>(p, o, z, ws, s)) != NOP_OK) return rc;
+        Params q = params_of<T>(d, p, o, z, ws);
+        q.out = o.y;
+        q.vec = d.points % 4 == 0 && aligned({o.x}, 4 * sizeof(IN));
+        rc = d.activation == NOP_ACT_GELU
+                 ? launch(k_block<T, IN, false, true>, grid, kThreads, p.smem, s, q, dev.status)
+                 : launch(k_block<T, IN, false, false>, grid, kThreads, p.smem, s, q, dev.status);
+        if (rc != NOP_OK || p.col0 + p.cols >= p.O) return rc;
+        if (!make_plan<T>(d, false, p.col0 + p.cols, &p)) return fail(NOP_E_UNSUPPORTED, kTooLarge);
+    }
+}
+
+template <class T>
+int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, const nop_gated_grads& g,
+                 const Sizes& z, char* ws, cudaStream_t s) {
+    Device dev;
+    int32_t rc = device(&dev);
+    if (rc != NOP_OK) return rc;
+    if ((rc = pack<T, true>(p, o, z, ws, s)) != NOP_OK) return rc;
+    const bool weights = g.gw_gate || g.gw_up || g.gw_down || g.gb_gate || g.gb_up || g.gb_down;
+    Params q = params_of<T>(d, p, o, z, ws);
+    q.gy = g.gy;
+    q.out = g.gx;
+    q.z = weights ? ws + z.z : nullptr;
+    q.zs = z.slab_tiles * TP;
+    q.vec = d.points % 4 == 0 && aligned({o.x, g.gy}, 4 * sizeof(T));
+    WParams w{};
+    w.z = ws + z.z;
+    w.x = o.x;
+    w.gy = g.gy;
+    w.zs = q.zs;
+    w.partial = reinterpret_cast<float*>(ws + z.partial);
+    w.sums = g.gb_gate || g.gb_up || g.gb_down ? reinterpret_cast<double*>(ws + z.sums) : nullptr;
+    w.C = p.C;
+    w.H = p.H;
+    w.O = p.O;
+    w.P = q.P;
+    w.points = q.points;
+    w.nC = (int)ceil_div(p.C, 128);
+    w.nO = (int)ceil_div(p.O, 128);
+    w.mX = (int)ceil_div(2 * p.H, 128);
+    w.mH = (int)ceil_div(p.H, 128);
+    w.splits = z.splits;
+    w.vec = d.points % 8 == 0 && aligned({o.x, g.gy}, 16);
+    const int64_t slab = weights ? z.slab_tiles : z.tiles;
+    constexpr int wsmem = kWStages * 2 * Form<T>::SPL * 128 * Form<T>::KC * 2 + (int)sizeof(WBars);
+    for (int64_t t = 0; t < z.tiles; t += slab) {
+        q.tile0 = (int)t;
+        q.tiles = (int)std::min<int64_t>(slab, z.tiles - t);
+        const unsigned grid = (unsigned)std::min<int64_t>(q.tiles, dev.sms);
+        rc = d.activation == NOP_ACT_GELU ? launch(k_block<T, T, true, true>, grid, kThreads, p.smem, s, q, dev.status)
+                                          : launch(k_block<T, T, true, false>, grid, kThreads, p.smem, s, q, dev.status);
+        if (rc != NOP_OK) return rc;
+        if (!weights) continue;
+        w.first = (uint32_t)(t * TP);
+        w.pieces = q.tiles * (TP / Form<T>::KC);
+        w.accumulate = t > 0;
+        rc = launch(k_wgrad<T>, (unsigned)(z.splits * z.wtiles), kWThreads, wsmem, s, w, dev.status);
+        if (rc != NOP_OK) return rc;
+    }
+    // dL/dx of the channels past the first launch's: the products again, without the scratch
+    while (g.gx && p.col0 + p.cols < p.C) {
+        if (!make_plan<T>(d, true, p.col0 + p.cols, &p)) return fail(NOP_E_UNSUPPORTED, kTooLarge);
+        if ((rc = pack<T, true>(p, o, z, ws, s)) != NOP_OK) return rc;
+        Params r = params_of<T>(d, p, o, z, ws);
+        r.gy = q.gy;
+        r.out = q.out;
+        r.vec = q.vec;
+        const unsigned grid = (unsigned)std::min<int64_t>(z.tiles, dev.sms);
+        rc = d.activation == NOP_ACT_GELU ? launch(k_block<T, T, true, true>, grid, kThreads, p.smem, s, r, dev.status)
+                                          : launch(k_block<T, T, true, false>, grid, kThreads, p.smem, s, r, dev.status);
+        if (rc != NOP_OK) return rc;
+    }
+    if (!weights) return NOP_OK;
+    const unsigned vecs = w.sums ? (unsigned)ceil_div(2 * p.H + p.O, 128) : 0;
+    k_finish<T><<<3 * p.H + vecs, 128, 0, s>>>(w, static_cast<T*>(g.gw_gate), static_cast<T*>(g.gw_up),
+                                               static_cast<T*>(g.gw_down), static_cast<T*>(g.gb_gate),
+                                               static_cast<T*>(g.gb_up), static_cast<T*>(g.gb_down));
+    NOP_CUDA_TRY(cudaGetLastError());
+    return NOP_OK;
+}
+
+int32_t check_operands(const nop_gated_desc& d, const nop_gated_operands* o) {
+    if (!o) return fail(NOP_E_INVALID, "operands are NULL");
+    if (!o->x || !o->w_gate || !o->w_up || !o->w_down)
+        return fail(NOP_E_INVALID, "x, w_gate, w_up and w_down must be non-NULL");
+    if (d.x_dtype == NOP_DTYPE_E4M3 && !o->x_scale) return fail(NOP_E_INVALID, "an e4m3 field needs x_scale");
+    const uintptr_t size = d.dtype == NOP_DTYPE_FP32 ? 4 : 2;
+    if ((d.x_dtype != NOP_DTYPE_E4M3 && (uintptr_t)o->x % size) || (uintptr_t)o->x_scale % 4 ||
+        !aligned({o->w_gate, o->w_up, o->w_down, o->b_gate, o->b_up, o->b_down, o->y}, size))
+        return fail(NOP_E_ALIGNMENT, "a pointer is not aligned to its type");
+    return NOP_OK;
+}
+
+}  // namespace gated
+}  // namespace nop
+
+using namespace nop;
+
+extern "C" {
+
+int32_t nop_gated_workspace_size(const nop_gated_desc* d, int32_t backward, size_t* bytes) {
+    const int32_t rc = gated::check(d);
+    if (rc != NOP_OK) return rc;
+    if (!bytes) return fail(NOP_E_INVALID, "bytes is NULL");
+    return gated::by_type(d->dtype, [&](auto t) {
+        using T = decltype(t);
+        gated::Plan p;
+        if (!gated::make_plan<T>(*d, backward != 0, 0, &p))
+            return fail(NOP_E_UNSUPPORTED, gated::kTooLarge);
+        *bytes = gated::sizes_of<T>(*d, p, backward != 0).bytes;
+        return (int32_t)NOP_OK;
+    });
+}
+
+int32_t nop_gated_forward(const nop_gated_desc* d, const nop_gated_operands* o, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+    int32_t rc = gated::check(d);
+    if (rc != NOP_OK) return rc;
+    if (d->batch == 0 || d->points == 0) return NOP_OK;
+    if ((rc = gated::check_operands(*d, o)) != NOP_OK) return rc;
+    if (!o->y) return fail(NOP_E_INVALID, "y must be non-NULL");
+    return gated::by_type(d->dtype, [&](auto t) {
+        using T = decltype(t);
+        gated::Plan p;
+        if (!gated::make_plan<T>(*d, false, 0, &p))
+            return fail(NOP_E_UNSUPPORTED, gated::kTooLarge);
+        const gated::Sizes z = gated::sizes_of<T>(*d, p, false);
+        if (!workspace || workspace_bytes < z.bytes) return fail(NOP_E_WORKSPACE, "workspace missing or too small");
+        if ((uintptr_t)workspace % 256) return fail(NOP_E_ALIGNMENT, "the workspace must be 256-byte aligned");
+        char* ws = static_cast<char*>(workspace);
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if constexpr (sizeof(T) == 2) {
+            if (d->x_dtype == NOP_DTYPE_E4M3) return gated::forward<T, uint8_t>(*d, p, *o, z, ws, s);
+        }
+        return gated::forward<T, T>(*d, p, *o, z, ws, s);
+    });
+}
+
+int32_t nop_gated_backward(const nop_gated_desc* d, const nop_gated_operands* o, const nop_gated_grads* g,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    int32_t rc = gated::check(d);
+    if (rc != NOP_OK) return rc;
+    if (d->x_dtype != d->dtype) return fail(NOP_E_UNSUPPORTED, "the backward takes no e4m3 field");
+    if (!g) return fail(NOP_E_INVALID, "grads are NULL");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (d->batch == 0 || d->points == 0) {  // no points: the weights' gradients are zero
+        const size_t size = d->dtype == NOP_DTYPE_FP32 ? 4 : 2;
+        const size_t h = d->hidden, c = d->channels, n = d->out_channels;
+        for (auto [ptr, count] : {std::pair<void*, size_t>{g->gw_gate, h * c}, {g->gw_up, h * c}, {g->gw_down, n * h},
+                                  {g->gb_gate, h}, {g->gb_up, h}, {g->gb_down, n}})
+            if (ptr) NOP_CUDA_TRY(cudaMemsetAsync(ptr, 0, count * size, s));
+        return NOP_OK;
+    }
+    if ((rc = gated::check_operands(*d, o)) != NOP_OK) return rc;
+    if (!g->gy) return fail(NOP_E_INVALID, "gy must be non-NULL");
+    if (!gated::aligned({g->gy, g->gx, g->gw_gate, g->gw_up, g->gw_down, g->gb_gate, g->gb_up, g->gb_down},
+                        d->dtype == NOP_DTYPE_FP32 ? 4 : 2))
+        return fail(NOP_E_ALIGNMENT, "a pointer is not aligned to its type");
+    return gated::by_type(d->dtype, [&](auto t) {
+        using T = decltype(t);
+        gated::Plan p;
+        if (!gated::make_plan<T>(*d, true, 0, &p))
+            return fail(NOP_E_UNSUPPORTED, gated::kTooLarge);
+        const gated::Sizes z = gated::sizes_of<T>(*d, p, true);
+        if (!workspace || workspace_bytes < z.bytes) return fail(NOP_E_WORKSPACE, "workspace missing or too small");
+        if ((uintptr_t)workspace % 256) return fail(NOP_E_ALIGNMENT, "the workspace must be 256-byte aligned");
+        return gated::backward<T>(*d, p, *o, *g, z, static_cast<char*>(workspace), s);
+    });
+}
+
+}  // extern "C"

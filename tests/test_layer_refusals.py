@@ -97,3 +97,94 @@ def test_clip_pointers():
     assert call(dst=None, norm=None) == -1 and call(src=0) == -1 and call(dst=0) == -1
     assert call(src=66) == -3 and call(dst=66) == -3 and call(ws=68) == -3
     assert call(ws=None) == -4 and call(ws_bytes=8) == -4
+
+
+def gated_ops(c=4, h=6, o=3, dtype=f32):
+    return [fake(h, c, dtype=dtype), fake(h, c, dtype=dtype), fake(o, h, dtype=dtype)]
+
+
+def test_gated_mlp_refuses_cpu_tensors():
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        nb.gated_mlp(fake(1, 4, 5), *gated_ops())
+
+
+@pytest.mark.parametrize("case, error", [
+    (dict(activation="relu"), ValueError),
+    (dict(x=(4,)), ValueError),
+    (dict(x=(1, 5, 7)), ValueError),
+    (dict(w_up=(6, 5)), ValueError),
+    (dict(w_down=(3, 7)), ValueError),
+    (dict(w_gate=(6, 4, 2)), ValueError),
+    (dict(b_gate=(5,)), ValueError),
+    (dict(b_down=(6,)), ValueError),
+    (dict(x=(1, 300, 7), w_gate=(6, 300), w_up=(6, 300)), ValueError),
+    (dict(w_down=(257, 6)), ValueError),
+    (dict(w_gate=(16385, 4), w_up=(16385, 4), w_down=(3, 16385)), ValueError),
+    (dict(x=(1, 4, 7), dtype_x=torch.bfloat16), TypeError),
+    (dict(dtype=torch.float64), TypeError),
+    (dict(x_scale=(1, 1, 7)), TypeError),
+    (dict(dtype_x=torch.float8_e4m3fn, x_scale=(1, 1, 7)), TypeError),
+])
+def test_gated_mlp_arguments(case, error, monkeypatch):
+    """The checks run on the host; the tensors only claim to be on a device."""
+    from neuraloperator_b200 import gated
+
+    dtype = case.get("dtype", f32)
+    t = {"x": (1, 4, 7), "w_gate": (6, 4), "w_up": (6, 4), "w_down": (3, 6), "b_gate": None, "b_up": None,
+         "b_down": None, "x_scale": None, **{k: v for k, v in case.items() if isinstance(v, tuple)}}
+    t = {k: None if v is None else torch.empty(v, dtype=dtype, device="meta") for k, v in t.items()}
+    if "dtype_x" in case:
+        t["x"] = t["x"].to(case["dtype_x"])
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
+    with pytest.raises(error):
+        gated._check(t["x"], t["w_gate"], t["w_up"], t["w_down"], (t["b_gate"], t["b_up"], t["b_down"]),
+                     case.get("activation", "silu"), t["x_scale"])
+
+
+def gated_desc(**over):
+    d = _lib.NopGatedDesc(_lib.ABI_VERSION, 0, 0, 0, 2, 16, 8, 12, 8, 0)
+    for k, v in over.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(), 0), (dict(abi_version=7), -1), (dict(dtype=3), -1), (dict(x_dtype=1), -1), (dict(x_dtype=3), -2),
+    (dict(dtype=1, x_dtype=3), 0), (dict(activation=2), -1), (dict(batch=-1), -1), (dict(points=-1), -1),
+    (dict(channels=0), -1), (dict(hidden=0), -1), (dict(out_channels=0), -1), (dict(channels=257), -2),
+    (dict(out_channels=257), -2), (dict(hidden=16385), -2), (dict(batch=1 << 16, points=1 << 16), -2)])
+def test_gated_descriptor(over, code):
+    lib, size = _lib.library(), ctypes.c_size_t()
+    assert lib.nop_gated_workspace_size(gated_desc(**over), 0, size) == code, _lib.last_error()
+
+
+def test_gated_plan_takes_every_width():
+    """Every admitted combination of channels, hidden width, type and pass has a plan."""
+    lib, size = _lib.library(), ctypes.c_size_t()
+    for dtype in range(3):
+        for c in (1, 16, 17, 64, 127, 128, 129, 250, 256):
+            for o in (1, 16, 100, 128, 129, 256):
+                for h in (1, 16, 17, 48, 64, 65, 100, 129, 500, 16384):
+                    for backward in (0, 1):
+                        d = gated_desc(dtype=dtype, x_dtype=dtype, channels=c, out_channels=o, hidden=h)
+                        assert lib.nop_gated_workspace_size(d, backward, size) == 0, (dtype, c, o, h, backward)
+
+
+def test_gated_pointers():
+    lib, size = _lib.library(), ctypes.c_size_t()
+    d = gated_desc()
+    assert lib.nop_gated_workspace_size(d, 0, size) == 0
+    full = dict(x=512, w_gate=512, w_up=512, w_down=512, y=512)
+    ops = lambda **kw: _lib.NopGatedOperands(**{**full, **kw})  # noqa: E731
+    fwd = lambda o, ws=512, n=None: lib.nop_gated_forward(d, o, ws, size.value if n is None else n, None)  # noqa: E731
+    for name in full:
+        assert fwd(ops(**{name: None})) == -1, name
+    assert fwd(ops(x=514)) == -3 and fwd(ops(b_up=513)) == -3 and fwd(ops(), ws=520) == -3
+    assert fwd(ops(), ws=None) == -4 and fwd(ops(), n=8) == -4
+    assert lib.nop_gated_forward(gated_desc(dtype=1, x_dtype=3), ops(), 512, 1 << 30, None) == -1  # no scales
+    g = _lib.NopGatedGrads(gy=None, gx=512)
+    assert lib.nop_gated_backward(d, ops(), g, 512, 1 << 30, None) == -1
+    assert lib.nop_gated_backward(d, ops(), None, 512, 1 << 30, None) == -1
+    assert lib.nop_gated_backward(d, ops(), _lib.NopGatedGrads(gy=512, gx=513), 512, 1 << 30, None) == -3
+    assert lib.nop_gated_backward(d, ops(), _lib.NopGatedGrads(gy=512, gx=512), 512, 8, None) == -4
+    assert lib.nop_gated_backward(gated_desc(dtype=1, x_dtype=3), ops(), g, 512, 1 << 30, None) == -2
