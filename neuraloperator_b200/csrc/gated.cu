@@ -33,18 +33,21 @@
 // columns of the banks.  Weights are packed once a call (k_pack) into images that a bulk copy brings into shared
 // memory whole; they stay there for the whole kernel when they fit, and stream through a ring otherwise.
 //
-// The weight gradients contract over points, which are contiguous in every operand: k_wgrad reads dg, du, h (left
-// by k_block in a scratch [3 H][points of a slab]), x and e, splits the points over the CTAs and leaves partial
+// The weight gradients contract over points, which are contiguous in every operand: k_wgrad reads dg, du, h,
+// x and e (left by k_block in a scratch [tile][3 H + C + O][128 points]: with rows as long as the slab every store
+// went to a page of its own, 100 cycles each; x and e in their own places would need aligned rows), splits the points over the CTAs and leaves partial
 // sums that k_finish adds in a fixed order.  Because of the truncation a long sum is cut: every kPromote pieces the
 // epilogue warps add the accumulator (fp32: and the smaller products' own) to registers.
-// The scratch is made and consumed slab by slab, sized to stay in L2.
+// The scratch is made and consumed slab by slab.
 //
 // Every wait is bounded: on expiry the kernel records NOP_DEVICE_MMA_TIMEOUT in the status word, all roles leave
 // their loops, copies and MMAs in flight are waited for (bounded) and the tensor memory is freed.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mix_tc.cuh"
 
@@ -96,7 +99,8 @@ struct Plan {
     int resident;              // 1: all weight images stay in shared memory
     int a_slot, b_slot;        // bytes
     int job_bytes;             // packed weight bytes of one chunk
-    int o_a, o_b, o_bar, smem;
+    int vec_smem;              // 1: the biases have a copy in shared memory
+    int o_a, o_b, o_vec, o_bar, smem;
 };
 
 struct Params {
@@ -104,10 +108,9 @@ struct Params {
     const void* gy;            // backward: e
     const float* scale;        // e4m3 x: one a point
     const char* packed;
-    const float *bg, *bu, *b2; // fp32, padded with zeros (b2: the output's, forward)
+    const float* bias;         // the biases of g, u and (forward) of the output: fp32, padded with zeros
     void* out;                 // y, or dL/dx (may be NULL)
-    void* z;                   // backward: [3 H][zs] dg, du, h (may be NULL)
-    int64_t zs;
+    void* z;                   // backward: [tile][3 H + C + O][128] dg, du, h, x, e (may be NULL)
     uint32_t P, points;        // a sample's points, all points
     int tile0, tiles;          // tiles of this launch
     int vec;                   // 4 points a load
@@ -125,16 +128,44 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t addr, int sbo) {
 __device__ __forceinline__ uint32_t idesc_of(uint32_t fmt, int N) {
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(TP >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-    tc::mma_bf16(d, a, b, idesc, acc ? 1u : 0u);
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+// One lane of the (converged) warp.  The MMA warp runs its loops with all lanes and only predicates the MMAs and
+// commits on it: its descriptors and addresses then stay in uniform registers.  With the loops inside a one-lane
+// branch every MMA cost its warp 105 to 120 cycles, more than the tensor core needs for most of them.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%6, %6, %6, %6}, p;\n\t}"
         :
-        : "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u), "r"(0), "r"(0), "r"(0), "r"(0)
+        : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u), "r"(leader), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%6, %6, %6, %6}, p;\n\t}"
+        :
+        : "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u), "r"(leader), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(tc::smem_u32(bar)),
+        "r"(leader)
         : "memory");
 }
 __device__ __forceinline__ void ld16(uint32_t taddr, float (&v)[16]) {
@@ -180,48 +211,66 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// two neighbouring K elements as one word of each image
-template <class T> __device__ __forceinline__ void images(float v0, float v1, uint32_t (&w)[Form<T>::SPL]);
-template <> __device__ __forceinline__ void images<__nv_bfloat16>(float v0, float v1, uint32_t (&w)[1]) {
-    w[0] = tc::pack_bf16(v0, v1);
+// Two neighbouring K elements as one word of each image.  Pairs of values go through packed fp32 arithmetic
+// wherever there is some: the epilogue warps are bound by their instruction count.
+template <class T> __device__ __forceinline__ void images(float2 v, uint32_t (&w)[Form<T>::SPL]);
+template <> __device__ __forceinline__ void images<__nv_bfloat16>(float2 v, uint32_t (&w)[1]) {
+    w[0] = tc::pack_bf16(v.x, v.y);
 }
-template <> __device__ __forceinline__ void images<__half>(float v0, float v1, uint32_t (&w)[1]) {
-    const __half2 h = __floats2half2_rn(v0, v1);
+template <> __device__ __forceinline__ void images<__half>(float2 v, uint32_t (&w)[1]) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
     w[0] = *reinterpret_cast<const uint32_t*>(&h);
 }
-template <> __device__ __forceinline__ void images<float>(float v0, float v1, uint32_t (&w)[3]) {
+template <> __device__ __forceinline__ void images<float>(float2 v, uint32_t (&w)[3]) {
     // v = a + b + c, each part the rounding of what is left (the differences are exact)
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-        w[i] = tc::pack_bf16(v0, v1);
-        v0 -= __uint_as_float(w[i] << 16);
-        v1 -= __uint_as_float(w[i] & 0xFFFF0000u);
+        w[i] = tc::pack_bf16(v.x, v.y);
+        if (i < 2) v = __ffma2_rn(make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)),
+                                  make_float2(-1.f, -1.f), v);
     }
 }
 
-// act(g) and act'(g).  SiLU: g s, s (1 + g (1 - s)), s = 1 / (1 + exp(-g)).  GELU: g P(g), P(g) + g p(g) with the
-// normal distribution function P from erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + q x), Abramowitz &
-// Stegun, Handbook of Mathematical Functions (1964), eq. 7.1.26 (|error| <= 1.5e-7); its exponential is also the
-// density's.
-constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// act(g) and act'(g) of two values.  SiLU: g s, s (1 + g (1 - s)), s = 1 / (1 + exp(-g)).  GELU: g P(g),
+// P(g) + g p(g) with the normal distribution function P from erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2),
+// t = 1 / (1 + q x), Abramowitz & Stegun, Handbook of Mathematical Functions (1964), eq. 7.1.26 (|error| <= 1.5e-7);
+// its exponential is also the density's.  Reciprocal and exponential are the special-function unit's (2^-22 or so):
+// of an infinite exponential the reciprocal is 0, which is the limit.
 template <bool GELU>
-__device__ __forceinline__ float activation(float g, float& slope) {
+__device__ __forceinline__ float2 activation(float2 g, float2& slope) {
     if (!GELU) {
-        const float s = __fdividef(1.f, 1.f + exp2f(-kLog2e * g));
-        slope = s * fmaf(g, 1.f - s, 1.f);
-        return g * s;
+        const float2 t = __fmul2_rn(g, both(-1.4426950408889634f));
+        const float2 d = __fadd2_rn(make_float2(exp2_approx(t.x), exp2_approx(t.y)), both(1.f));
+        const float2 s = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+        const float2 a = __fmul2_rn(g, s);
+        slope = __ffma2_rn(a, __ffma2_rn(s, both(-1.f), both(1.f)), s);
+        return a;
     }
-    const float x = fabsf(g) * 0.70710678118654752f;
-    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    const float e = exp2f(-kLog2e * x * x);
-    float s = fmaf(t, 1.061405429f, -1.453152027f);
-    s = fmaf(t, s, 1.421413741f);
-    s = fmaf(t, s, -0.284496736f);
-    s = fmaf(t, s, 0.254829592f);
-    const float tail = 0.5f * s * t * e;          // P(-|g|)
-    const float cdf = g < 0.f ? tail : 1.f - tail;
-    slope = fmaf(g * 0.3989422804014327f, e, cdf);
-    return g * cdf;
+    const float2 x = make_float2(fabsf(g.x), fabsf(g.y));  // |g| = sqrt(2) times erfc's argument
+    const float2 d = __ffma2_rn(x, both(0.3275911f * 0.70710678118654752f), both(1.f));
+    const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    const float2 q = __fmul2_rn(__fmul2_rn(g, g), both(-0.5f * 1.4426950408889634f));
+    const float2 e = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+    float2 s = __ffma2_rn(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+    s = __ffma2_rn(t, s, both(0.5f * 1.421413741f));
+    s = __ffma2_rn(t, s, both(0.5f * -0.284496736f));
+    s = __ffma2_rn(t, s, both(0.5f * 0.254829592f));
+    const float2 tail = __fmul2_rn(__fmul2_rn(s, t), e);   // P(-|g|)
+    const float2 cdf = make_float2(g.x < 0.f ? tail.x : 1.f - tail.x, g.y < 0.f ? tail.y : 1.f - tail.y);
+    slope = __ffma2_rn(__fmul2_rn(g, both(0.3989422804014327f)), e, cdf);
+    return __fmul2_rn(g, cdf);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -299,7 +348,7 @@ k_pack(Plan pl, const T* __restrict__ wg, const T* __restrict__ wu, const T* __r
         }
         uint32_t img[4][SPL];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) images<T>(v[2 * e], v[2 * e + 1], img[e]);
+        for (int e = 0; e < 4; ++e) images<T>(make_float2(v[2 * e], v[2 * e + 1]), img[e]);
 #pragma unroll
         for (int s = 0; s < SPL; ++s)
             *reinterpret_cast<uint4*>(packed + off + s * rows * pw * 2) =
@@ -379,14 +428,14 @@ __device__ __forceinline__ void store_item(const Item<IN>& it, char* slot, int c
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if constexpr (sizeof(IN) == 4) {
-                images<T>(__uint_as_float(it.w[8 * e + i]), __uint_as_float(it.w[8 * e + 4 + i]), img[e]);
+                images<T>(make_float2(__uint_as_float(it.w[8 * e + i]), __uint_as_float(it.w[8 * e + 4 + i])), img[e]);
             } else if constexpr (sizeof(IN) == 2) {
                 img[e][0] = __byte_perm(it.w[4 * e + i / 2], it.w[4 * e + 2 + i / 2], i & 1 ? 0x7632 : 0x5410);
             } else {
                 const uint32_t two = __byte_perm(it.w[2 * e], it.w[2 * e + 1], (uint32_t)(i | (4 + i) << 4));
                 const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffff), __NV_E4M3);
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                images<T>(f.x, f.y, img[e]);  // exact
+                images<T>(f, img[e]);  // exact
             }
         }
         char* at = base + (row >> 3) * kAGroup + (row & 7) * 16;
@@ -394,6 +443,31 @@ __device__ __forceinline__ void store_item(const Item<IN>& it, char* slot, int c
         for (int s = 0; s < SPL; ++s)
             *reinterpret_cast<uint4*>(at + s * steps * (16 * kAGroup)) =
                 make_uint4(img[0][s], img[1][s], img[2][s], img[3][s]);
+    }
+}
+
+// the item's channels below `rows` as rows of 128 points
+template <class T>
+__device__ __forceinline__ void copy_item(const Item<T>& it, T* __restrict__ z, int c0, int rows, int lane, bool vec) {
+    constexpr int W = Item<T>::W;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (c0 + e >= rows) break;
+        T* to = z + (c0 + e) * TP;
+        if (vec) {
+            if constexpr (W == 4)
+                *reinterpret_cast<uint4*>(to + 4 * lane) =
+                    make_uint4(it.w[4 * e], it.w[4 * e + 1], it.w[4 * e + 2], it.w[4 * e + 3]);
+            else
+                *reinterpret_cast<uint2*>(to + 4 * lane) = make_uint2(it.w[2 * e], it.w[2 * e + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (W == 4) to[lane + 32 * i] = __uint_as_float(it.w[4 * e + i]);
+                else
+                    reinterpret_cast<uint16_t*>(to)[lane + 32 * i] = (uint16_t)(it.w[2 * e + i / 2] >> (16 * (i & 1)));
+            }
+        }
     }
 }
 
@@ -415,7 +489,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
     const Plan& pl = p.pl;
     Bars& bar = *reinterpret_cast<Bars*>(sm + pl.o_bar);
     volatile int* abort_flag = &bar.abort_flag;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
         for (int i = 0; i < kMaxA; ++i) {
             tc::mbar_init(&bar.full_a[i], kProd);
@@ -436,6 +511,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         bar.abort_flag = 0;
     }
+    const float* vec = p.bias;
+    if (pl.vec_smem) {  // k_pack's values, read by every middle: out of L2 they cost it 600 cycles a time
+        float* v = reinterpret_cast<float*>(sm + pl.o_vec);
+        for (int i = tid; i < 2 * pl.NH * pl.nJ + pl.N2; i += kThreads) v[i] = __ldg(p.bias + i);
+        vec = v;
+    }
+    const float *bias_g = vec, *bias_u = vec + pl.NH * pl.nJ, *bias_2 = vec + 2 * pl.NH * pl.nJ;
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc::smem_u32(&bar.tmem))
                      : "memory");
@@ -444,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = bar.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, bar.tmem, 0);
     auto give_up = [&]() {
         *abort_flag = 1;
         atomicExch(status, tc::kStatusMmaTimeout);
@@ -486,6 +568,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
 #pragma unroll
             for (int i = 0; i < NI; ++i)
                 if ((w + 4 * i) * 8 < pw) store_item<T, IN>(it[i], s, w + 4 * i, pw / 16, lane, p.vec);
+            if constexpr (BWD) {  // x and e go to the scratch too, once a tile
+                const int k = a / nA;
+                if (p.z && (pl.reuse || k % pl.nJ == 0)) {
+                    const bool is_x = kc < pl.nKx;
+                    const int c0 = (is_x ? kc : kc - pl.nKx) * KC, rows = is_x ? pl.C : pl.O;
+                    const int tile = (pl.reuse ? k : k / pl.nJ) * (int)gridDim.x + (int)blockIdx.x;
+                    T* z = static_cast<T*>(p.z) +
+                           ((int64_t)tile * (3 * pl.H + pl.C + pl.O) + 3 * pl.H + (is_x ? 0 : pl.C)) * TP;
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) copy_item<T>(it[i], z, c0 + (w + 4 * i) * 8, rows, lane, p.vec);
+                }
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&bar.full_a[slot]);
@@ -542,92 +636,118 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
         }
     } else if (warp == kMma) {
         // ------------------------------ MMA issue ------------------------------
-        if (lane == 0 && jobs > 0) {
+        if (jobs > 0) {
+            const uint32_t leader = elect_one();
             const uint32_t sa = tc::smem_u32(sm + pl.o_a), sb = tc::smem_u32(sm + pl.o_b);
             constexpr uint32_t fmt = Form<T>::kFmt;
-            int q = 0;
-            bool ok = !pl.resident || wait(&bar.full_b[0], 0);
-            // the images of the next weight piece (`at`: its place among its chunk's, when resident)
-            auto weights = [&](int j, int at) -> uint32_t {
-                if (pl.resident) return sb + (uint32_t)(j * pl.job_bytes + at);
-                if (!wait(&bar.full_b[q % pl.nb], (uint32_t)(q / pl.nb) & 1)) ok = false;
-                return sb + (uint32_t)((q % pl.nb) * pl.b_slot);
+            const uint32_t id_g = idesc_of(fmt, 2 * pl.NH), id_f = idesc_of(fmt, pl.NH), id_2 = idesc_of(fmt, pl.N2);
+            auto all = [&](uint64_t* b, uint32_t parity) -> bool {  // the warp stays together
+                return __all_sync(0xffffffffu, wait(b, parity));
+            };
+            int qs = 0, a0 = 0;            // weight slot; slot of the job's (reuse: the tile's) first A piece
+            uint32_t qp = 0, ap = 0;       // their phases
+            bool ok = !pl.resident || all(&bar.full_b[0], 0);
+            // the images of the next weight piece (`at`: its place among all of them, when resident)
+            auto weights = [&](int at) -> uint32_t {
+                if (pl.resident) return sb + (uint32_t)at;
+                if (!all(&bar.full_b[qs], qp)) ok = false;
+                return sb + (uint32_t)(qs * pl.b_slot);
             };
             auto weights_done = [&]() {
                 if (pl.resident) return;
-                tc::mma_commit(&bar.empty_b[q % pl.nb]);
-                ++q;
+                commit(&bar.empty_b[qs], leader);
+                if (++qs == pl.nb) {
+                    qs = 0;
+                    qp ^= 1;
+                }
             };
-            // D (columns d ..) (+)= A piece from shared memory x B piece of N rows
-            auto product_ss = [&](uint32_t d, uint32_t a0, uint32_t b0, int N, int pw, bool acc) {
+            // D (columns d ..) (+)= A piece from shared memory x B piece of N rows; the smaller products first
+            auto product_ss = [&](uint32_t d, uint32_t at, uint32_t bt, uint32_t id, int N, int pw, bool acc) {
                 const int steps = pw / 16;
-                const uint32_t id = idesc_of(fmt, N);
                 uint64_t da[SPL], db[SPL];
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
-                    da[s] = desc_of(a0 + s * steps * (16 * kAGroup), kAGroup);
-                    db[s] = desc_of(b0 + s * N * pw * 2, 256);
+                    da[s] = desc_of(at + s * steps * (16 * kAGroup), kAGroup);
+                    db[s] = desc_of(bt + s * N * pw * 2, 256);
                 }
-                for (int ks = 0; ks < steps; ++ks) {  // the smaller products
+                const uint32_t bstep = N * 2;
+                if constexpr (NP > 1) {
 #pragma unroll
-                    for (int i = 1; i < NP; ++i) {
-                        mma_ss(d, da[Passes<SPL>::a(i)] + ks * (kAGroup), db[Passes<SPL>::b(i)] + ks * (N * 2), id, acc);
-                        acc = true;
+                    for (int ks = 0; ks < KC / 16; ++ks) {
+                        if (ks >= steps) break;
+#pragma unroll
+                        for (int i = 1; i < NP; ++i)
+                            mma_ss(d, da[Passes<SPL>::a(i)] + ks * kAGroup, db[Passes<SPL>::b(i)] + ks * bstep, id,
+                                   acc || ks > 0 || i > 1, leader);
                     }
                 }
-                for (int ks = 0; ks < steps; ++ks) {
-                    mma_ss(d, da[0] + ks * kAGroup, db[0] + ks * (N * 2), id, acc);
-                    acc = true;
+#pragma unroll
+                for (int ks = 0; ks < KC / 16; ++ks) {
+                    if (ks >= steps) break;
+                    mma_ss(d, da[0] + ks * kAGroup, db[0] + ks * bstep, id, NP > 1 || acc || ks > 0, leader);
                 }
             };
             // ... x A images in tensor memory; image s of the K step of hidden group g at column col[s] + 16 g; the
             // smaller products in the N columns after D's
-            auto product_ts = [&](uint32_t d, const uint32_t (&col)[SPL], uint32_t b0, int N, int pw, bool acc, int g0) {
-                const uint32_t id = idesc_of(fmt, N);
+            auto product_ts = [&](uint32_t d, const uint32_t (&col)[SPL], uint32_t bt, int N, int pw, bool acc, int g0) {
                 uint64_t db[SPL];
 #pragma unroll
-                for (int s = 0; s < SPL; ++s) db[s] = desc_of(b0 + s * N * pw * 2, 256);
-                for (int ks = 0; ks < pw / 16; ++ks) {
+                for (int s = 0; s < SPL; ++s) db[s] = desc_of(bt + s * N * pw * 2, 256);
+                const uint32_t bstep = N * 2;
+#pragma unroll
+                for (int ks = 0; ks < KC / 16; ++ks) {
+                    if (ks >= pw / 16) break;
 #pragma unroll
                     for (int i = 0; i < NP; ++i)
-                        mma_ts(i ? d + N : d, col[Passes<SPL>::a(i)] + 16 * (g0 + ks), db[Passes<SPL>::b(i)] + ks * (N * 2),
-                               id, i > 1 || acc);
-                    acc = true;
+                        mma_ts(i ? d + N : d, col[Passes<SPL>::a(i)] + 16 * (g0 + ks), db[Passes<SPL>::b(i)] + ks * bstep,
+                               id_2, i > 1 || acc || ks > 0, leader);
                 }
             };
+            int j1 = 0, j2 = 0, k2 = 0;    // chunk of the first and of the second product, tile of the second
             for (int J = 0; J <= jobs && ok; ++J) {
+                const int b = J & 1;
                 if (J < jobs) {  // first product of job J
-                    const int b = J & 1, j = J % pl.nJ, k = J / pl.nJ;
-                    if (J >= 2 && !wait(&bar.g2[b], (uint32_t)((J >> 1) - 1) & 1)) break;
+                    if (J >= 2 && !all(&bar.g2[b], (uint32_t)((J >> 1) - 1) & 1)) break;
                     fence_after();
                     const uint32_t d = tmem + b * d1w;
-                    int at = 0;
-                    for (int kc = 0; kc < nA && ok; ++kc) {
+                    const bool last = j1 == pl.nJ - 1;
+                    int at = j1 * pl.job_bytes, slot = a0;
+                    uint32_t phase = ap;
+                    for (int kc = 0; kc < nA; ++kc) {
                         const bool is_x = kc < pl.nKx;
-                        const int a = (pl.reuse ? k : J) * nA + kc, slot = a % pl.na;
                         const int pw = is_x ? piece_k(pl.Kx, KC, kc) : piece_k(pl.Ky, KC, kc - pl.nKx);
                         const int N = is_x ? 2 * pl.NH : pl.NH;
-                        if (!wait(&bar.full_a[slot], (uint32_t)(a / pl.na) & 1)) ok = false;
-                        const uint32_t wb = weights(j, at);
+                        if (!all(&bar.full_a[slot], phase)) ok = false;
+                        const uint32_t wb = weights(at);
                         if (!ok) break;
                         fence_after();
-                        product_ss(is_x ? d : d + 2 * pl.NH, sa + slot * pl.a_slot, wb, N, pw, kc != 0 && kc != pl.nKx);
+                        product_ss(is_x ? d : d + 2 * pl.NH, sa + slot * pl.a_slot, wb, is_x ? id_g : id_f, N, pw,
+                                   kc != 0 && kc != pl.nKx);
                         at += N * pw * 2 * SPL;
                         weights_done();
-                        if (!pl.reuse || j == pl.nJ - 1) tc::mma_commit(&bar.empty_a[slot]);
+                        if (!pl.reuse || last) commit(&bar.empty_a[slot], leader);
+                        if (++slot == pl.na) {
+                            slot = 0;
+                            phase ^= 1;
+                        }
                     }
                     if (!ok) break;
-                    tc::mma_commit(&bar.d1[b]);
+                    commit(&bar.d1[b], leader);
+                    if (!pl.reuse || last) {
+                        a0 = slot;
+                        ap = phase;
+                    }
+                    j1 = last ? 0 : j1 + 1;
                 }
                 if (J > 0) {  // second product of job J - 1
-                    const int q1 = J - 1, b = q1 & 1, j = q1 % pl.nJ, k = q1 / pl.nJ;
-                    if (!wait(&bar.mid[b], (uint32_t)(q1 >> 1) & 1)) break;
-                    if (j == 0 && k > 0 && !wait(&bar.d2_free, (uint32_t)(k - 1) & 1)) break;
+                    if (!all(&bar.mid[b ^ 1], (uint32_t)((J - 1) >> 1) & 1)) break;
+                    if (j2 == 0 && k2 > 0 && !all(&bar.d2_free, (uint32_t)(k2 - 1) & 1)) break;
                     fence_after();
-                    const uint32_t d = tmem + b * d1w;
-                    int at = pl.NH * (2 * pl.Kx + pl.Ky) * 2 * SPL;
+                    const uint32_t d = tmem + (b ^ 1) * d1w;
+                    int at = j2 * pl.job_bytes + pl.NH * (2 * pl.Kx + pl.Ky) * 2 * SPL;
+#pragma unroll
                     for (int m = 0; m < (BWD ? 2 : 1); ++m) {
-                        uint32_t col[SPL];  // the places that the middle gave the images (k_block's epilogue)
+                        uint32_t col[SPL];  // the places that the middle gave the images
                         if constexpr (SPL == 1) {
                             col[0] = d + m * pl.NH;
                         } else {
@@ -635,24 +755,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                             col[1] = m ? d + 2 * pl.NH : d + 8;
                             col[2] = m ? d + 2 * pl.NH + 8 : d + pl.NH;
                         }
-                        for (int kc = 0; kc < pl.nH; ++kc) {
+                        for (int kc = 0; kc < pl.nH && ok; ++kc) {
                             const int pw = piece_k(pl.NH, KC, kc);
-                            const uint32_t wb = weights(j, at);
+                            const uint32_t wb = weights(at);
                             if (!ok) break;
                             fence_after();
-                            product_ts(d2, col, wb, pl.N2, pw, j != 0 || m != 0 || kc != 0, kc * (KC / 16));
+                            product_ts(d2, col, wb, pl.N2, pw, j2 != 0 || m != 0 || kc != 0, kc * (KC / 16));
                             at += pl.N2 * pw * 2 * SPL;
                             weights_done();
                         }
-                        if (!ok) break;
                     }
                     if (!ok) break;
-                    tc::mma_commit(&bar.g2[b]);
-                    if (j == pl.nJ - 1) tc::mma_commit(&bar.d2);
+                    commit(&bar.g2[b ^ 1], leader);
+                    if (++j2 == pl.nJ) {
+                        commit(&bar.d2, leader);
+                        j2 = 0;
+                        ++k2;
+                    }
                 }
             }
             // every MMA issued has completed before the tensor memory is freed (bounded)
-            tc::mma_commit(&bar.drain);
+            commit(&bar.drain, leader);
             tc::mbar_wait(&bar.drain, 0, nullptr);
         }
     } else if (warp < kEpi) {
@@ -678,31 +801,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                 wait_ld(vg);
                 wait_ld(vu);
                 const int h0 = j * pl.NH + 16 * g;
-                const float4* bg = reinterpret_cast<const float4*>(p.bg + h0);
-                const float4* bu = reinterpret_cast<const float4*>(p.bu + h0);
+                const float4* bg = reinterpret_cast<const float4*>(bias_g + h0);
+                const float4* bu = reinterpret_cast<const float4*>(bias_u + h0);
+                float2 g2[8], u2[8];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float4 a = __ldg(bg + i), c = __ldg(bu + i);
-                    vg[4 * i] = fmaf(vg[4 * i], sc, a.x);
-                    vg[4 * i + 1] = fmaf(vg[4 * i + 1], sc, a.y);
-                    vg[4 * i + 2] = fmaf(vg[4 * i + 2], sc, a.z);
-                    vg[4 * i + 3] = fmaf(vg[4 * i + 3], sc, a.w);
-                    vu[4 * i] = fmaf(vu[4 * i], sc, c.x);
-                    vu[4 * i + 1] = fmaf(vu[4 * i + 1], sc, c.y);
-                    vu[4 * i + 2] = fmaf(vu[4 * i + 2], sc, c.z);
-                    vu[4 * i + 3] = fmaf(vu[4 * i + 3], sc, c.w);
+                    const float4 a = bg[i], c = bu[i];
+                    g2[2 * i] = __ffma2_rn(make_float2(vg[4 * i], vg[4 * i + 1]), both(sc), make_float2(a.x, a.y));
+                    g2[2 * i + 1] = __ffma2_rn(make_float2(vg[4 * i + 2], vg[4 * i + 3]), both(sc), make_float2(a.z, a.w));
+                    u2[2 * i] = __ffma2_rn(make_float2(vu[4 * i], vu[4 * i + 1]), both(sc), make_float2(c.x, c.y));
+                    u2[2 * i + 1] = __ffma2_rn(make_float2(vu[4 * i + 2], vu[4 * i + 3]), both(sc), make_float2(c.z, c.w));
                 }
                 if constexpr (!BWD) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float slope;
-                        vg[i] = activation<GELU>(vg[i], slope) * vu[i];
-                    }
                     uint32_t w[SPL][8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
+                        float2 slope;
                         uint32_t t[SPL];
-                        images<T>(vg[2 * i], vg[2 * i + 1], t);
+                        images<T>(__fmul2_rn(activation<GELU>(g2[i], slope), u2[i]), t);
 #pragma unroll
                         for (int s = 0; s < SPL; ++s) w[s][i] = t[s];
                     }
@@ -715,27 +831,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                     float vf[16];
                     ld16(d + 2 * pl.NH + 16 * g, vf);
                     wait_ld(vf);
-                    T* z = static_cast<T*>(p.z) + (int64_t)h0 * p.zs + (int64_t)(tile - p.tile0) * TP + row;
+                    T* z = static_cast<T*>(p.z) + ((int64_t)(tile - p.tile0) * (3 * pl.H + pl.C + pl.O) + h0) * TP + row;
+                    T *zu = z + pl.H * TP, *zh = zu + pl.H * TP;
+                    const int left = p.z ? pl.H - h0 : 0;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float slope;
-                        const float a = activation<GELU>(vg[i], slope);
-                        const float h = a * vu[i];
-                        // points past the last one hold a product of zeros: their rows of the scratch are zeros
-                        vg[i] = valid ? vf[i] * vu[i] * slope : 0.f;
-                        vu[i] = valid ? vf[i] * a : 0.f;
-                        if (p.z && h0 + i < pl.H) {
-                            z[(int64_t)i * p.zs] = from_f<T>(vg[i]);
-                            z[(int64_t)(pl.H + i) * p.zs] = from_f<T>(vu[i]);
-                            z[(int64_t)(2 * pl.H + i) * p.zs] = from_f<T>(valid ? h : 0.f);
+                    for (int i = 0; i < 8; ++i) {
+                        float2 slope;
+                        const float2 a = activation<GELU>(g2[i], slope);
+                        // points past the last one are zeros in the scratch
+                        const float2 f = valid ? make_float2(vf[2 * i], vf[2 * i + 1]) : both(0.f);
+                        const float2 h = valid ? __fmul2_rn(a, u2[i]) : both(0.f);
+                        g2[i] = __fmul2_rn(__fmul2_rn(f, u2[i]), slope);
+                        u2[i] = __fmul2_rn(f, a);
+                        if (2 * i < left) {
+                            z[2 * i * TP] = from_f<T>(g2[i].x);
+                            zu[2 * i * TP] = from_f<T>(u2[i].x);
+                            zh[2 * i * TP] = from_f<T>(h.x);
+                        }
+                        if (2 * i + 1 < left) {
+                            z[(2 * i + 1) * TP] = from_f<T>(g2[i].y);
+                            zu[(2 * i + 1) * TP] = from_f<T>(u2[i].y);
+                            zh[(2 * i + 1) * TP] = from_f<T>(h.y);
                         }
                     }
                     uint32_t w[2][SPL][8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         uint32_t t[SPL], r[SPL];
-                        images<T>(vg[2 * i], vg[2 * i + 1], t);
-                        images<T>(vu[2 * i], vu[2 * i + 1], r);
+                        images<T>(g2[i], t);
+                        images<T>(u2[i], r);
 #pragma unroll
                         for (int s = 0; s < SPL; ++s) {
                             w[0][s][i] = t[s];
@@ -780,12 +904,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] += c[i];
                 }
+                if constexpr (!BWD) {  // all loads before the stores, which might alias them for all the compiler knows
+                    const float4* b2 = reinterpret_cast<const float4*>(bias_2 + 16 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 c = b2[i];
+                        v[4 * i] += c.x;
+                        v[4 * i + 1] += c.y;
+                        v[4 * i + 2] += c.z;
+                        v[4 * i + 3] += c.w;
+                    }
+                }
                 if (!valid || !p.out) continue;
                 T* yg = y + (int64_t)(16 * g) * p.P;
+                const int left = pl.cols - 16 * g;
+                if (left >= 16) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (!BWD) v[i] += __ldg(p.b2 + 16 * g + i);
-                    if (16 * g + i < pl.cols) yg[(int64_t)i * p.P] = from_f<T>(v[i]);
+                    for (int i = 0; i < 16; ++i) yg[(int64_t)i * p.P] = from_f<T>(v[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (i < left) yg[(int64_t)i * p.P] = from_f<T>(v[i]);
                 }
             }
             fence_before();
@@ -809,95 +948,79 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
 // ------------------------------------------------------------------------------------------------
 // weight gradients
 // ------------------------------------------------------------------------------------------------
-constexpr int kWThreads = 32 * 16;            // warps 0..7 epilogue (warp 0 also issues the MMAs), 8..15 producers
+constexpr int kWork = 4;                      // warps 8..11: fp32 splitting, row sums (warps 0..7: accumulators)
+constexpr int kWMma = 8 + kWork, kWLoad = kWMma + 1;
+constexpr int kWThreads = 32 * (kWLoad + 1);
 constexpr int kPromote = 8;                   // pieces an accumulator runs before it goes to registers
-constexpr int kWStages = 3;
+constexpr int kImages = 2;                    // fp32: stages of split operands
+
+// A piece is 128 bytes of points of up to 128 rows of each operand, as a 128-byte-swizzled tensor copy leaves them:
+// for 16-bit types that is the MMA's own K-major layout and the pieces are multiplied as they land.
+template <class T> struct WForm {
+    static constexpr int KC = 128 / (int)sizeof(T);
+    static constexpr int STAGES = sizeof(T) == 4 ? 3 : 6;
+    static constexpr int RAW = 2 * 128 * 128;                        // A rows, then B rows
+    static constexpr int IMG = sizeof(T) == 4 ? 128 * KC * 2 : 0;    // one image of one operand
+    static constexpr int SPLIT = 2 * Form<T>::SPL * IMG;
+    static constexpr int BODY = STAGES * RAW + (sizeof(T) == 4 ? kImages * SPLIT : 0);
+};
 
 struct WParams {
-    const void *z, *x, *gy;
-    int64_t zs;
     float* partial;            // [split][tile][128][128]
-    double* sums;              // [split][2 H + O] row sums of dg, du and e
+    double* sums;              // [split][2 H + O] row sums of dg, du and e (may be NULL)
     int C, H, O;
-    uint32_t P, points;        // a sample's points, all points
-    uint32_t first;            // the slab's first point
+    int rows;                  // rows of a tile of the scratch
     int pieces;                // pieces of KC points in the slab
     int splits;
     int nC, nO;                // column tiles of x and of e
     int mX, mH;                // row tiles of [dg; du] and of h
     int accumulate;            // add to the partial sums of the slabs before
-    int vec;                   // 8 points of x and e a wide load
 };
 
 struct WBars {
-    uint64_t full[kWStages], empty[kWStages], acc[2], acc_free[2], drain;
+    uint64_t raw[6], raw_free[6], img[kImages], img_free[kImages], acc[2], acc_free[2], drain;
     uint32_t tmem;
     int abort_flag;
 };
 
-// 8 points of one row
-template <class T> struct Eight {
-    static constexpr int W = (int)sizeof(T) * 2;
-    uint32_t w[W];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = 0;
-    }
-    __device__ __forceinline__ void load_wide(const T* a) {
-#pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(a) + i);
-            w[4 * i] = q.x;
-            w[4 * i + 1] = q.y;
-            w[4 * i + 2] = q.z;
-            w[4 * i + 3] = q.w;
-        }
-    }
-    __device__ __forceinline__ void put(int i, const T* a) {
-        if constexpr (sizeof(T) == 4) w[i] = __ldg(reinterpret_cast<const uint32_t*>(a));
-        else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(a)) << (16 * (i & 1));
-    }
-    __device__ __forceinline__ float get(int i) const {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
-        else {
-            const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-            return to_f(*reinterpret_cast<const T*>(&h));
-        }
-    }
-};
-
-template <class T>
-__device__ __forceinline__ void store_eight(const Eight<T>& v, char* at, int image_bytes) {
-    constexpr int SPL = Form<T>::SPL;
-    if constexpr (SPL == 1) {
-        *reinterpret_cast<uint4*>(at) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
-    } else {
-        uint32_t img[4][SPL];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) images<T>(v.get(2 * e), v.get(2 * e + 1), img[e]);
-#pragma unroll
-        for (int s = 0; s < SPL; ++s)
-            *reinterpret_cast<uint4*>(at + s * image_bytes) = make_uint4(img[0][s], img[1][s], img[2][s], img[3][s]);
-    }
+__device__ __forceinline__ uint64_t desc_128b(uint32_t addr) {  // K-major rows of 128 bytes, 128-byte swizzle
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// CTA = (tile, split).  Tile: 128 rows of the scratch (rows of [dg; du] against channels of x, rows of h against
-// channels of e) x 128 channels; K: the split's share of the slab's points.
+// CTA = (tile, split).  Tile: 128 rows of the scratch (rows of [dg; du] against rows of x, rows of h against rows of
+// e) x up to 128 columns; K: the split's share of the slab's points.
 template <class T>
-__global__ void __launch_bounds__(kWThreads, 1) k_wgrad(const __grid_constant__ WParams p, int* __restrict__ status) {
-    constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N;
-    constexpr int IMG = 128 * KC * 2, SLOT = 2 * SPL * IMG;   // A images, then B images
-    constexpr int DW = SPL == 3 ? 256 : 128;                  // columns of an accumulator (and the smaller products')
+__global__ void __launch_bounds__(kWThreads, 1)
+k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mx,
+        const __grid_constant__ CUtensorMap me, const __grid_constant__ WParams p, int* __restrict__ status) {
+    using W = WForm<T>;
+    constexpr int SPL = Form<T>::SPL, KC = W::KC, NP = Passes<SPL>::N, S = W::STAGES;
+    constexpr bool kSplit = SPL > 1;
+    constexpr int DW = kSplit ? 256 : 128;      // columns of an accumulator (and the smaller products')
     extern __shared__ __align__(1024) char sm[];
-    WBars& bar = *reinterpret_cast<WBars*>(sm + kWStages * SLOT);
+    WBars& bar = *reinterpret_cast<WBars*>(sm + W::BODY);
     volatile int* abort_flag = &bar.abort_flag;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int tiles = p.mX * p.nC + p.mH * p.nO;
+    const int tile = (int)blockIdx.x % tiles, split = (int)blockIdx.x / tiles;
+    const bool of_x = tile < p.mX * p.nC;
+    const int mt = of_x ? tile / p.nC : (tile - p.mX * p.nC) / p.nO, nt = of_x ? tile % p.nC : (tile - p.mX * p.nC) % p.nO;
+    const int a_rows = (of_x ? 2 * p.H : p.H) - mt * 128;    // rows left from the tile's first
+    const int b_rows = (of_x ? p.C : p.O) - nt * 128;
+    const int n = imin(128, up16(b_rows));
+    const int k0 = (int)((int64_t)p.pieces * split / p.splits), k1 = (int)((int64_t)p.pieces * (split + 1) / p.splits);
+    const int steps = k1 - k0, runs = (steps + kPromote - 1) / kPromote;
+    const bool want_a = p.sums && of_x && nt == 0, want_b = p.sums && !of_x && mt == 0;
+    const bool working = kSplit || want_a || want_b;
     if (tid == 0) {
-        for (int i = 0; i < kWStages; ++i) {
-            tc::mbar_init(&bar.full[i], 8);
-            tc::mbar_init(&bar.empty[i], 1);
+        for (int i = 0; i < S; ++i) {
+            tc::mbar_init(&bar.raw[i], 1);
+            tc::mbar_init(&bar.raw_free[i], kSplit ? kWork : working ? kWork + 1 : 1);
         }
         for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&bar.img[i], kWork);
+            tc::mbar_init(&bar.img_free[i], 1);
             tc::mbar_init(&bar.acc[i], 1);
             tc::mbar_init(&bar.acc_free[i], 8);
         }
@@ -914,113 +1037,155 @@ __global__ void __launch_bounds__(kWThreads, 1) k_wgrad(const __grid_constant__ 
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = bar.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, bar.tmem, 0);
     auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
         if (tc::mbar_wait(b, parity, abort_flag)) return true;
         *abort_flag = 1;
         atomicExch(status, tc::kStatusMmaTimeout);
         return false;
     };
-    const int tiles = p.mX * p.nC + p.mH * p.nO;
-    const int tile = (int)blockIdx.x % tiles, split = (int)blockIdx.x / tiles;
-    const bool of_x = tile < p.mX * p.nC;
-    const int mt = of_x ? tile / p.nC : (tile - p.mX * p.nC) / p.nO, nt = of_x ? tile % p.nC : (tile - p.mX * p.nC) % p.nO;
-    const int a_rows = of_x ? 2 * p.H - mt * 128 : p.H - mt * 128;     // rows left from the tile's first
-    const int b_rows = of_x ? p.C - nt * 128 : p.O - nt * 128;
-    const int n = imin(128, up16(b_rows));
-    const int k0 = (int)((int64_t)p.pieces * split / p.splits), k1 = (int)((int64_t)p.pieces * (split + 1) / p.splits);
-    const int steps = k1 - k0, runs = (steps + kPromote - 1) / kPromote;
+    char* split_at = sm + S * W::RAW;
 
-    if (warp >= 8 && warp < 16) {
-        // ------------------------------ producers ------------------------------
-        // lane: row lane % 8 of an 8-row group, 16-byte column lane / 8 (+ 4); warp w: groups w and w + 8
-        constexpr int NI = KC / 32;
-        const int w = warp - 8, r8 = lane & 7, ch0 = lane >> 3;
-        const int bc = of_x ? p.C : p.O;
-        const T* za = static_cast<const T*>(p.z) + (int64_t)((of_x ? 0 : 2 * p.H) + mt * 128) * p.zs;
-        const T* xb = static_cast<const T*>(of_x ? p.x : p.gy) + (int64_t)nt * 128 * p.P;
-        double sum_a[2] = {0.0, 0.0}, sum_b[2] = {0.0, 0.0};
-        const bool want_a = p.sums && of_x && nt == 0, want_b = p.sums && !of_x && mt == 0;
-        Eight<T> ca[2][NI], cb[2][NI], na[2][NI], nb[2][NI];
-        auto load = [&](Eight<T>(&ia)[2][NI], Eight<T>(&ib)[2][NI], int k) {
+    if (warp == kWLoad) {
+        // ------------------------------ scratch -> shared memory ------------------------------
+        if (lane == 0) {
+            const CUtensorMap* mb = of_x ? &mx : &me;
+            const int a0 = (of_x ? 0 : 2 * p.H) + mt * 128, b0 = 3 * p.H + (of_x ? 0 : p.C) + nt * 128;
+            const uint32_t bytes = (uint32_t)(128 + imin(128, of_x ? p.C : p.O)) * 128;
+            int k = 0;
+            for (; k < steps; ++k) {
+                const int slot = k % S, use = k / S;
+                if (use > 0 && !wait(&bar.raw_free[slot], (uint32_t)(use - 1) & 1)) break;
+                const int at = (k0 + k) * KC, t = at / TP, c = at % TP;
+                const uint32_t dst = tc::smem_u32(sm + slot * W::RAW);
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(&bar.raw[slot])),
+                             "r"(bytes)
+                             : "memory");
+                auto copy = [&](uint32_t to, const CUtensorMap* m, int row) {
+                    asm volatile(
+                        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+                        "%3}], [%4];" ::"r"(to),
+                        "l"(reinterpret_cast<uint64_t>(m)), "r"(c), "r"(row), "r"(tc::smem_u32(&bar.raw[slot]))
+                        : "memory");
+                };
+                copy(dst, &ma, t * p.rows + a0);
+                copy(dst + W::RAW / 2, mb, t * p.rows + b0);
+            }
+            for (int i = 0; i < S && i < k; ++i)  // no copy outlives the CTA (bounded)
+                tc::mbar_wait(&bar.raw[(k - 1 - i) % S], (uint32_t)((k - 1 - i) / S) & 1, nullptr);
+        }
+    } else if (warp >= 8 && warp < kWMma) {
+        // ------------------------------ splitting and row sums: a thread has a row of each operand ----------------
+        const int r = tid - 256;
+        double sum = 0.0;
+        auto row_of = [&](const char* raw, float (&v)[KC]) {
+            const char* row = raw + r * 128;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const uint32_t q = (uint32_t)(k0 + k) * KC + (ch0 + 4 * i) * 8;  // point within the slab
-                const uint32_t pt = p.first + q;
-                const uint32_t b = pt < p.points ? pt / p.P : 0, o = pt < p.points ? pt - b * p.P : 0;
+            for (int c = 0; c < 8; ++c) {
+                const uint4 q = *reinterpret_cast<const uint4*>(row + ((c ^ (r & 7)) * 16));
+                const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const int r = (w + 8 * g) * 8 + r8;
-                    if (r < a_rows) ia[g][i].load_wide(za + (int64_t)r * p.zs + q);
-                    else ia[g][i].zero();
-                    if (r >= b_rows || pt >= p.points) {
-                        ib[g][i].zero();
-                    } else if (p.vec) {
-                        ib[g][i].load_wide(xb + ((int64_t)b * bc + r) * p.P + o);
-                    } else {
-                        ib[g][i].zero();
-                        uint32_t bb = b, oo = o;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if (pt + e < p.points) ib[g][i].put(e, xb + ((int64_t)bb * bc + r) * p.P + oo);
-                            if (++oo == p.P) {
-                                oo = 0;
-                                ++bb;
-                            }
-                        }
-                    }
-                }
+                for (int i = 0; i < KC / 8; ++i) v[c * (KC / 8) + i] = to_f(e[i]);
             }
         };
-        auto put = [&](const Eight<T>(&ia)[2][NI], const Eight<T>(&ib)[2][NI], int k) -> bool {
-            const int slot = k % kWStages, use = k / kWStages;
-            if (use > 0 && !wait(&bar.empty[slot], (uint32_t)(use - 1) & 1)) return false;
-            char* s = sm + slot * SLOT;
+        auto add = [&](const float (&v)[KC]) {  // a piece's values in fp32, the pieces in 64 bits
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                float ta = 0.f, tb = 0.f;
+            for (int i = 0; i < KC; ++i) s[i % 4] += v[i];
+            sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+        };
+        for (int k = 0; working && k < steps; ++k) {
+            const int slot = k % S;
+            if (!wait(&bar.raw[slot], (uint32_t)(k / S) & 1)) break;
+            const char* raw = sm + slot * W::RAW;
+            float v[KC];
+            if constexpr (kSplit) {
+                const int si = k % kImages, use = k / kImages;
+                if (use > 0 && !wait(&bar.img_free[si], (uint32_t)(use - 1) & 1)) break;
 #pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const int ch = ch0 + 4 * i, off = (ch >> 1) * (128 * 32) + (w + 8 * g) * 256 + (ch & 1) * 128 + r8 * 16;
-                    store_eight<T>(ia[g][i], s + off, IMG);
-                    if ((w + 8 * g) * 8 < n) store_eight<T>(ib[g][i], s + SPL * IMG + off, IMG);
-                    if (want_a) {
+                for (int o = 0; o < 2; ++o) {
+                    if (o && r >= n) break;
+                    row_of(raw + o * (W::RAW / 2), v);
+                    char* to = split_at + si * W::SPLIT + o * SPL * W::IMG + (r >> 3) * 256 + (r & 7) * 16;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) ta += ia[g][i].get(e);
+                    for (int ch = 0; ch < KC / 8; ++ch) {
+                        uint32_t img[4][SPL];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) images<T>(make_float2(v[8 * ch + 2 * e], v[8 * ch + 2 * e + 1]), img[e]);
+#pragma unroll
+                        for (int q = 0; q < SPL; ++q)
+                            *reinterpret_cast<uint4*>(to + q * W::IMG + (ch >> 1) * (128 * 32) + (ch & 1) * 128) =
+                                make_uint4(img[0][q], img[1][q], img[2][q], img[3][q]);
                     }
-                    if (want_b) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) tb += ib[g][i].get(e);
-                    }
+                    if (o ? want_b : want_a) add(v);
                 }
-                sum_a[g] += (double)ta;
-                sum_b[g] += (double)tb;
+            } else {
+                row_of(raw + (want_b ? W::RAW / 2 : 0), v);
+                add(v);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&bar.full[slot]);
-            return true;
-        };
-        if (steps > 0) load(ca, cb, 0);
-        for (int k = 0; k < steps; k += 2) {
-            if (k + 1 < steps) load(na, nb, k + 1);
-            if (!put(ca, cb, k)) break;
-            if (k + 1 >= steps) break;
-            if (k + 2 < steps) load(ca, cb, k + 2);
-            if (!put(na, nb, k + 1)) break;
-        }
-        if (want_a || want_b) {
-            double* out = p.sums + (int64_t)split * (2 * p.H + p.O) + (want_a ? mt * 128 : 2 * p.H + nt * 128);
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                double v = want_a ? sum_a[g] : sum_b[g];
-                v += __shfl_xor_sync(0xffffffffu, v, 8);
-                v += __shfl_xor_sync(0xffffffffu, v, 16);
-                const int r = (w + 8 * g) * 8 + r8;
-                if (lane < 8 && r < (want_a ? a_rows : b_rows)) out[r] = p.accumulate ? out[r] + v : v;
+            if (lane == 0) {
+                if (kSplit) tc::mbar_arrive(&bar.img[k % kImages]);
+                tc::mbar_arrive(&bar.raw_free[slot]);
             }
         }
-    } else if (warp < 8) {
+        if ((want_a && r < a_rows) || (want_b && r < b_rows)) {
+            double* out = p.sums + (int64_t)split * (2 * p.H + p.O) + (want_a ? mt * 128 : 2 * p.H + nt * 128) + r;
+            *out = p.accumulate ? *out + sum : sum;
+        }
+    } else if (warp == kWMma) {
+        // ------------------------------ MMA issue ------------------------------
+        const uint32_t leader = elect_one();
+        const uint32_t id = idesc_of(Form<T>::kFmt, n);
+        auto all = [&](uint64_t* b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+        constexpr int Q = kSplit ? kImages : S;
+        int slot = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int r = 0; r < runs && ok; ++r) {
+            const int buf = r & 1;
+            if (r >= 2 && !all(&bar.acc_free[buf], (uint32_t)((r >> 1) - 1) & 1)) break;
+            fence_after();
+            const int end = imin(steps, (r + 1) * kPromote);
+            for (int k = r * kPromote; k < end; ++k) {
+                if (!all(kSplit ? &bar.img[slot] : &bar.raw[slot], phase)) {
+                    ok = false;
+                    break;
+                }
+                fence_after();
+                const bool first = k == r * kPromote;
+                const uint32_t d = tmem + buf * DW;
+                if constexpr (kSplit) {
+                    const uint32_t at = tc::smem_u32(split_at + slot * W::SPLIT);
+                    const uint64_t a0 = desc_of(at, 256), b0 = desc_of(at + SPL * W::IMG, 256);
+#pragma unroll
+                    for (int ks = 0; ks < KC / 16; ++ks) {
+#pragma unroll
+                        for (int i = 0; i < NP; ++i)
+                            mma_ss(d + (i ? 128 : 0), a0 + (Passes<SPL>::a(i) * W::IMG + ks * 128 * 32) / 16,
+                                   b0 + (Passes<SPL>::b(i) * W::IMG + ks * 128 * 32) / 16, id, i > 1 || ks > 0 || !first,
+                                   leader);
+                    }
+                    commit(&bar.img_free[slot], leader);
+                } else {
+                    const uint32_t at = tc::smem_u32(sm + slot * W::RAW);
+                    const uint64_t a0 = desc_128b(at), b0 = desc_128b(at + W::RAW / 2);
+#pragma unroll
+                    for (int ks = 0; ks < KC / 16; ++ks) mma_ss(d, a0 + 2 * ks, b0 + 2 * ks, id, ks > 0 || !first, leader);
+                    commit(&bar.raw_free[slot], leader);
+                }
+                if (++slot == Q) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+            if (ok) commit(&bar.acc[buf], leader);
+        }
+        // every MMA issued has completed before the tensor memory is freed (bounded)
+        commit(&bar.drain, leader);
+        tc::mbar_wait(&bar.drain, 0, nullptr);
+    } else {
         // ------------------------------ accumulators -> registers -> partial sums ------------------------------
         const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
         float sum[4][16];   // groups of 16 columns half, half + 2, ...
@@ -1028,38 +1193,9 @@ __global__ void __launch_bounds__(kWThreads, 1) k_wgrad(const __grid_constant__ 
         for (int g = 0; g < 4; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sum[g][i] = 0.f;
-        // run r's MMAs (kPromote pieces into accumulator r & 1), by warp 0's first lane
-        const uint32_t s0 = tc::smem_u32(sm);
-        const uint32_t id = idesc_of(Form<T>::kFmt, n);
-        auto issue = [&](int r) {
-            const int buf = r & 1;
-            if (r >= 2 && !wait(&bar.acc_free[buf], (uint32_t)((r >> 1) - 1) & 1)) return;
-            fence_after();
-            bool acc = false;
-            for (int k = r * kPromote; k < imin(steps, (r + 1) * kPromote); ++k) {
-                const int slot = k % kWStages;
-                if (!wait(&bar.full[slot], (uint32_t)(k / kWStages) & 1)) return;
-                fence_after();
-                const uint32_t a0 = s0 + slot * SLOT, b0 = a0 + SPL * IMG;
-#pragma unroll
-                for (int ks = 0; ks < KC / 16; ++ks) {
-#pragma unroll
-                    for (int i = 0; i < NP; ++i)
-                        mma_ss(tmem + buf * DW + (i ? 128 : 0), desc_of(a0 + Passes<SPL>::a(i) * IMG + ks * 128 * 32, 256),
-                               desc_of(b0 + Passes<SPL>::b(i) * IMG + ks * 128 * 32, 256), id, i > 1 || acc);
-                    acc = true;
-                }
-                tc::mma_commit(&bar.empty[slot]);
-            }
-            tc::mma_commit(&bar.acc[buf]);
-        };
-        const bool issuer = tid == 0;
-        if (issuer && runs > 0) issue(0);
         bool ok = true;
         for (int r = 0; r < runs; ++r) {
             const int buf = r & 1;
-            if (issuer && r + 1 < runs) issue(r + 1);  // the tensor core works on r + 1 while r is read
-            __syncwarp();
             if (!wait(&bar.acc[buf], (uint32_t)(r >> 1) & 1)) {
                 ok = false;
                 break;
@@ -1086,10 +1222,6 @@ __global__ void __launch_bounds__(kWThreads, 1) k_wgrad(const __grid_constant__ 
             fence_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&bar.acc_free[buf]);
-        }
-        if (issuer) {  // every MMA issued has completed before the tensor memory is freed (bounded)
-            tc::mma_commit(&bar.drain);
-            tc::mbar_wait(&bar.drain, 0, nullptr);
         }
         if (ok && row < a_rows) {
             float* out = p.partial + ((int64_t)split * tiles + tile) * (128 * 128) + row * 128;
@@ -1179,7 +1311,9 @@ bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
     p.a_slot = (kx / 16) * 16 * kAGroup * SPL;
     p.b_slot = std::max(2 * p.NH * imin(KC, p.Kx), std::max(p.NH * imin(KC, p.Ky), p.N2 * kh)) * 2 * SPL;
     p.job_bytes = (p.NH * (2 * p.Kx + p.Ky) + (bwd ? 2 : 1) * p.N2 * p.NH) * 2 * SPL;
-    const int64_t room = kSmem - 1024 - (int64_t)sizeof(Bars);
+    const int vec = (2 * p.NH * p.nJ + p.N2) * 4;
+    p.vec_smem = vec <= 8192;  // hidden widths up to about 1000; wider ones read them from L1 or L2
+    const int64_t room = kSmem - 1024 - (int64_t)sizeof(Bars) - (p.vec_smem ? vec : 0);
     const int64_t all = (int64_t)p.nJ * p.job_bytes;
     const int nA = p.nKx + p.nKy;
     int64_t bytes;
@@ -1202,7 +1336,8 @@ bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
     p.o_a = 0;
     p.o_b = p.na * p.a_slot;
     p.o_b = (p.o_b + 127) & ~127;
-    p.o_bar = (int)((p.o_b + bytes + 127) & ~127);
+    p.o_vec = (int)((p.o_b + bytes + 127) & ~127);
+    p.o_bar = (p.o_vec + (p.vec_smem ? vec : 0) + 127) & ~127;
     p.smem = std::max(p.o_bar + (int)sizeof(Bars), 120 * 1024);  // one CTA an SM: it holds the whole tensor memory
     *out = p;
     return p.smem <= kSmem;
@@ -1232,12 +1367,14 @@ Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd) {
     s.vec = at;
     at += up(vectors);
     if (bwd) {
-        // the scratch of a slab stays within half of L2, in whole waves of 148 tiles
-        const int64_t tile_bytes = (int64_t)3 * p.H * TP * sizeof(T);
-        const int64_t waves = std::max<int64_t>(1, (int64_t)(64 << 20) / (148 * tile_bytes));
+        // The scratch of a slab: up to 512 MB, in whole waves of 148 tiles.  Slabs that stay in L2 save the scratch's
+        // trip through HBM but lose more to their launches' beginnings and ends: 64 MB slabs took 2207 us where
+        // 512 MB take 1646 (fp32, 64 channels, hidden 128, 2^20 points), and larger ones 1626.
+        const int64_t tile_bytes = (int64_t)(3 * p.H + p.C + p.O) * TP * sizeof(T);
+        const int64_t waves = std::max<int64_t>(1, (int64_t)(512 << 20) / (148 * tile_bytes));
         s.slab_tiles = std::min<int64_t>(s.tiles, 148 * waves);
         s.wtiles = (int)(ceil_div(2 * p.H, 128) * ceil_div(p.C, 128) + ceil_div(p.H, 128) * ceil_div(p.O, 128));
-        const int64_t pieces = s.slab_tiles * (TP / Form<T>::KC);
+        const int64_t pieces = s.slab_tiles * (TP / WForm<T>::KC);
         s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(148 / s.wtiles, pieces));
         s.z = at;
         at += up((size_t)s.slab_tiles * tile_bytes);
@@ -1298,6 +1435,26 @@ int32_t launch(K kernel, unsigned grid, int threads, int smem, cudaStream_t s, A
     return NOP_OK;
 }
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// rows of 128 points, boxes of 128 bytes x `box` rows
+template <class T>
+bool row_map(CUtensorMap* m, void* base, int64_t rows, int box) {
+    const EncodeTiled enc = reinterpret_cast<EncodeTiled>(tensor_map_encoder());
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)TP, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)TP * sizeof(T)};
+    const cuuint32_t sizes[2] = {(cuuint32_t)(128 / sizeof(T)), (cuuint32_t)box};
+    const cuuint32_t ones[2] = {1, 1};
+    const CUtensorMapDataType type = std::is_same<T, float>::value    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return enc(m, type, 2, base, dims, strides, sizes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool aligned(std::initializer_list<const void*> ps, uintptr_t to) {
     uintptr_t all = 0;
     for (const void* p : ps) all |= (uintptr_t)p;
@@ -1322,9 +1479,7 @@ Params params_of(const nop_gated_desc& d, const Plan& p, const nop_gated_operand
     q.x = o.x;
     q.scale = o.x_scale;
     q.packed = ws + z.packed;
-    q.bg = reinterpret_cast<const float*>(ws + z.vec);
-    q.bu = q.bg + p.NH * p.nJ;
-    q.b2 = q.bu + p.NH * p.nJ;
+    q.bias = reinterpret_cast<const float*>(ws + z.vec);
     q.P = (uint32_t)d.points;
     q.points = (uint32_t)(d.batch * d.points);
     q.tiles = (int)z.tiles;
@@ -1363,28 +1518,28 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
     q.gy = g.gy;
     q.out = g.gx;
     q.z = weights ? ws + z.z : nullptr;
-    q.zs = z.slab_tiles * TP;
     q.vec = d.points % 4 == 0 && aligned({o.x, g.gy}, 4 * sizeof(T));
     WParams w{};
-    w.z = ws + z.z;
-    w.x = o.x;
-    w.gy = g.gy;
-    w.zs = q.zs;
     w.partial = reinterpret_cast<float*>(ws + z.partial);
     w.sums = g.gb_gate || g.gb_up || g.gb_down ? reinterpret_cast<double*>(ws + z.sums) : nullptr;
     w.C = p.C;
     w.H = p.H;
     w.O = p.O;
-    w.P = q.P;
-    w.points = q.points;
+    w.rows = 3 * p.H + p.C + p.O;
     w.nC = (int)ceil_div(p.C, 128);
     w.nO = (int)ceil_div(p.O, 128);
     w.mX = (int)ceil_div(2 * p.H, 128);
     w.mH = (int)ceil_div(p.H, 128);
     w.splits = z.splits;
-    w.vec = d.points % 8 == 0 && aligned({o.x, g.gy}, 16);
+    CUtensorMap ma{}, mx{}, me{};
+    if (weights) {
+        const int64_t rows = z.slab_tiles * w.rows;
+        if (!row_map<T>(&ma, ws + z.z, rows, 128) || !row_map<T>(&mx, ws + z.z, rows, imin(128, p.C)) ||
+            !row_map<T>(&me, ws + z.z, rows, imin(128, p.O)))
+            return fail(NOP_E_CUDA, "cuTensorMapEncodeTiled(scratch) failed");
+    }
     const int64_t slab = weights ? z.slab_tiles : z.tiles;
-    constexpr int wsmem = kWStages * 2 * Form<T>::SPL * 128 * Form<T>::KC * 2 + (int)sizeof(WBars);
+    constexpr int wsmem = WForm<T>::BODY + (int)sizeof(WBars);
     for (int64_t t = 0; t < z.tiles; t += slab) {
         q.tile0 = (int)t;
         q.tiles = (int)std::min<int64_t>(slab, z.tiles - t);
@@ -1393,10 +1548,9 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
                                           : launch(k_block<T, T, true, false>, grid, kThreads, p.smem, s, q, dev.status);
         if (rc != NOP_OK) return rc;
         if (!weights) continue;
-        w.first = (uint32_t)(t * TP);
-        w.pieces = q.tiles * (TP / Form<T>::KC);
+        w.pieces = q.tiles * (TP / WForm<T>::KC);
         w.accumulate = t > 0;
-        rc = launch(k_wgrad<T>, (unsigned)(z.splits * z.wtiles), kWThreads, wsmem, s, w, dev.status);
+        rc = launch(k_wgrad<T>, (unsigned)(z.splits * z.wtiles), kWThreads, wsmem, s, ma, mx, me, w, dev.status);
         if (rc != NOP_OK) return rc;
     }
     // dL/dx of the channels past the first launch's: the products again, without the scratch
