@@ -34,9 +34,10 @@
 // memory whole; they stay there for the whole kernel when they fit, and stream through a ring otherwise.
 //
 // The weight gradients contract over points, which are contiguous in every operand: k_wgrad reads dg, du, h,
-// x and e (left by k_block in a scratch [tile][3 H + C + O][128 points]: with rows as long as the slab every store
-// went to a page of its own, 100 cycles each; x and e in their own places would need aligned rows), splits the points over the CTAs and leaves partial
-// sums that k_finish adds in a fixed order.  Because of the truncation a long sum is cut: every kPromote pieces the
+// x and e, all by tensor copies, splits the points over the CTAs and leaves partial sums that k_finish adds in a fixed
+// order.  k_block leaves dg, du and h in a scratch [tile][rows][128 points] (with rows as long as the slab every store
+// went to a page of its own, 100 cycles each), and x and e too, unless their samples are whole tiles on aligned rows
+// that a tensor copy can read in place.  Because of the truncation a long sum is cut: every kPromote pieces the
 // epilogue warps add the accumulator (fp32: and the smaller products' own) to registers.
 // The scratch is made and consumed slab by slab.
 //
@@ -55,11 +56,6 @@ namespace nop {
 namespace gated {
 
 constexpr int TP = 128;                       // points a tile
-constexpr int kEpi = 8;                       // warps 0..7: middle and output
-constexpr int kProd = 4;                      // warps 8..11: x (and e) into shared memory
-constexpr int kMma = kEpi + kProd;            // warp 12: MMA issue
-constexpr int kLoad = kMma + 1;               // warp 13: weight copies
-constexpr int kThreads = 32 * (kLoad + 1);
 constexpr int kSmem = 227 * 1024;
 constexpr int kAGroup = 272;                  // bytes between 8-row groups of an A image
 constexpr int kMaxA = 8, kMaxB = 8;           // ring slots at most
@@ -87,11 +83,18 @@ template <int SPL> struct Passes {
     __device__ static constexpr int b(int i) { return i == 1 || i == 3 ? 1 : i == 4 ? 2 : 0; }
 };
 
+// Warps of k_block: the middle's (and output's), the producers' (in groups of four that take the pieces in turn), MMA
+// issue, weight copies.
+template <bool BWD> struct Roles {
+    static constexpr int EPI = 8, GROUPS = BWD ? 1 : 2, MMA = EPI + 4 * GROUPS, LOAD = MMA + 1, THREADS = 32 * (LOAD + 1);
+};
+
 struct Plan {
     int C, H, O;               // channels of x, hidden width, channels of y
     int Kx, Ky;                // padded K of the first products (Ky: backward only, 0 otherwise)
     int cols, col0;            // channels of this launch's output, the first of them
     int N2;                    // padded columns of D2
+    int n_d2;                  // D2 buffers
     int NH, nJ;                // chunk width, chunks
     int nKx, nKy, nH;          // ring pieces: of x, of e, of a chunk in the second product
     int na, nb;                // ring slots (nb: streaming)
@@ -110,12 +113,21 @@ struct Params {
     const char* packed;
     const float* bias;         // the biases of g, u and (forward) of the output: fp32, padded with zeros
     void* out;                 // y, or dL/dx (may be NULL)
-    void* z;                   // backward: [tile][3 H + C + O][128] dg, du, h, x, e (may be NULL)
+    void* z;                   // backward: [tile][z_rows][128] dg, du, h (and x, e) (may be NULL)
+    int z_rows;                // 3 H, or 3 H + C + O
     uint32_t P, points;        // a sample's points, all points
+    uint32_t p_mul, p_shift;   // n / P = n p_mul >> p_shift for n < 2^31
     int tile0, tiles;          // tiles of this launch
     int vec;                   // 4 points a load
     Plan pl;
 };
+
+// The sample of point n.  A division by a run-time number costs some 100 cycles and several stood in every tile's
+// path: with s = ceil(log2 P) and m = ceil(2^(31 + s) / P) < 2^32, m P exceeds 2^(31 + s) by less than 2^s, so
+// n m / 2^(31 + s) exceeds n / P by less than 1 / P for n < 2^31 and has the same whole part.
+__device__ __forceinline__ uint32_t sample_of(const Params& p, uint32_t n) {
+    return (uint32_t)(((uint64_t)n * p.p_mul) >> p.p_shift);
+}
 
 __host__ __device__ inline int piece_k(int K, int KC, int kc) { return imin(KC, K - kc * KC); }
 
@@ -193,6 +205,18 @@ __device__ __forceinline__ void st8(uint32_t taddr, const uint32_t (&r)[8]) {
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
+// bounded wait (tc::mbar_wait) that first asks without reading the clock
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(tc::smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done || tc::mbar_wait(bar, parity, abort);
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -242,25 +266,28 @@ __device__ __forceinline__ float rcp_approx(float v) {
     return r;
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// two reciprocals for one special-function operation, which bound the middle (16 a cycle and SM): 1 / (x y) times the
+// other one
+__device__ __forceinline__ float2 rcp2(float2 v) { return __fmul2_rn(both(rcp_approx(v.x * v.y)), make_float2(v.y, v.x)); }
 
 // act(g) and act'(g) of two values.  SiLU: g s, s (1 + g (1 - s)), s = 1 / (1 + exp(-g)).  GELU: g P(g),
 // P(g) + g p(g) with the normal distribution function P from erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2),
 // t = 1 / (1 + q x), Abramowitz & Stegun, Handbook of Mathematical Functions (1964), eq. 7.1.26 (|error| <= 1.5e-7);
-// its exponential is also the density's.  Reciprocal and exponential are the special-function unit's (2^-22 or so):
-// of an infinite exponential the reciprocal is 0, which is the limit.
+// its exponential is also the density's.  Reciprocal and exponential are the special-function unit's (2^-22 or so).
 template <bool GELU>
 __device__ __forceinline__ float2 activation(float2 g, float2& slope) {
     if (!GELU) {
+        // below g = -41 the exponential is held at 2^60 (the product of two stays finite): |silu| < 1e-16 |g| there
         const float2 t = __fmul2_rn(g, both(-1.4426950408889634f));
-        const float2 d = __fadd2_rn(make_float2(exp2_approx(t.x), exp2_approx(t.y)), both(1.f));
-        const float2 s = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+        const float2 d = __fadd2_rn(make_float2(exp2_approx(fminf(t.x, 60.f)), exp2_approx(fminf(t.y, 60.f))), both(1.f));
+        const float2 s = rcp2(d);
         const float2 a = __fmul2_rn(g, s);
         slope = __ffma2_rn(a, __ffma2_rn(s, both(-1.f), both(1.f)), s);
         return a;
     }
     const float2 x = make_float2(fabsf(g.x), fabsf(g.y));  // |g| = sqrt(2) times erfc's argument
     const float2 d = __ffma2_rn(x, both(0.3275911f * 0.70710678118654752f), both(1.f));
-    const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    const float2 t = rcp2(d);
     const float2 q = __fmul2_rn(__fmul2_rn(g, g), both(-0.5f * 1.4426950408889634f));
     const float2 e = make_float2(exp2_approx(q.x), exp2_approx(q.y));
     float2 s = __ffma2_rn(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
@@ -373,7 +400,7 @@ __device__ __forceinline__ void load_item(Item<IN>& it, const IN* __restrict__ s
     if (p.vec) {
         const uint32_t n = n0 + 4 * lane;
         const bool ok = n < p.points;
-        const uint32_t b = ok ? n / p.P : 0;
+        const uint32_t b = ok ? sample_of(p, n) : 0;
         const IN* s = src + (int64_t)b * C * p.P + (ok ? n - b * p.P : 0) + (int64_t)c0 * p.P;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -401,7 +428,7 @@ __device__ __forceinline__ void load_item(Item<IN>& it, const IN* __restrict__ s
     for (int i = 0; i < 4; ++i) {
         const uint32_t n = n0 + lane + 32 * i;
         if (n >= p.points) continue;
-        const uint32_t b = n / p.P;
+        const uint32_t b = sample_of(p, n);
         const IN* s = src + (int64_t)b * C * p.P + (n - b * p.P) + (int64_t)c0 * p.P;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -446,6 +473,16 @@ __device__ __forceinline__ void store_item(const Item<IN>& it, char* slot, int c
     }
 }
 
+// Two rows of 16-bit values, this thread's point in both (one word), as words of two points: of two neighbouring
+// lanes the even one writes the first row and the odd one the second.
+template <class T>
+__device__ __forceinline__ void store_rows(T* at, uint32_t two, int lane, int left) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, two, 1);
+    const bool odd = lane & 1;
+    const uint32_t word = odd ? __byte_perm(other, two, 0x7632) : __byte_perm(two, other, 0x5410);
+    if (left > (odd ? 1 : 0)) *reinterpret_cast<uint32_t*>(at + (odd ? TP - 1 : 0)) = word;
+}
+
 // the item's channels below `rows` as rows of 128 points
 template <class T>
 __device__ __forceinline__ void copy_item(const Item<T>& it, T* __restrict__ z, int c0, int rows, int lane, bool vec) {
@@ -477,13 +514,16 @@ __device__ __forceinline__ void copy_item(const Item<T>& it, T* __restrict__ z, 
 // barriers, by index into the barrier area
 struct Bars {
     uint64_t full_a[kMaxA], empty_a[kMaxA], full_b[kMaxB], empty_b[kMaxB];
-    uint64_t d1[2], mid[2], g2[2], d2, d2_free, drain;
+    uint64_t d1[2], mid[2], g2[2], d2[2], d2_free[2], drain;
     uint32_t tmem;
     int abort_flag;
 };
 
 template <class T, class IN, bool BWD, bool GELU>
-__global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ Params p, int* __restrict__ status) {
+__global__ void __launch_bounds__(Roles<BWD>::THREADS, 1)
+k_block(const __grid_constant__ Params p, int* __restrict__ status) {
+    constexpr int kEpi = Roles<BWD>::EPI, kMma = Roles<BWD>::MMA, kLoad = Roles<BWD>::LOAD;
+    constexpr int kThreads = Roles<BWD>::THREADS, kGroups = Roles<BWD>::GROUPS;
     constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N;
     extern __shared__ __align__(1024) char sm[];
     const Plan& pl = p.pl;
@@ -493,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
         for (int i = 0; i < kMaxA; ++i) {
-            tc::mbar_init(&bar.full_a[i], kProd);
+            tc::mbar_init(&bar.full_a[i], 4);
             tc::mbar_init(&bar.empty_a[i], 1);
         }
         for (int i = 0; i < kMaxB; ++i) {
@@ -504,9 +544,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
             tc::mbar_init(&bar.d1[i], 1);
             tc::mbar_init(&bar.mid[i], kEpi);
             tc::mbar_init(&bar.g2[i], 1);
+            tc::mbar_init(&bar.d2[i], 1);
+            tc::mbar_init(&bar.d2_free[i], kEpi);
         }
-        tc::mbar_init(&bar.d2, 1);
-        tc::mbar_init(&bar.d2_free, kEpi);
         tc::mbar_init(&bar.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         bar.abort_flag = 0;
@@ -532,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
         atomicExch(status, tc::kStatusMmaTimeout);
     };
     auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
-        if (tc::mbar_wait(b, parity, abort_flag)) return true;
+        if (wait_for(b, parity, abort_flag)) return true;
         give_up();
         return false;
     };
@@ -541,41 +581,60 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
     const int jobs = my * pl.nJ;
     const int nA = pl.nKx + pl.nKy;                       // A pieces of a job
     const int d1w = (BWD ? 3 : 2) * pl.NH;                // columns of a D1 buffer
-    const uint32_t d2 = tmem + 2 * d1w;
+    const int d2w = pl.N2 * (SPL == 3 ? 2 : 1);           // columns of a D2 buffer (D2c after D2)
+    const uint32_t d2_0 = tmem + 2 * d1w;
+    // D2 buffer of this CTA's tile k, and how often it was used before
+    auto d2_buf = [&](int k) { return pl.n_d2 == 2 ? k & 1 : 0; };
+    auto d2_use = [&](int k) { return pl.n_d2 == 2 ? k >> 1 : k; };
     auto tile_at = [&](int k) { return (uint32_t)(p.tile0 + (int)blockIdx.x + k * (int)gridDim.x); };
 
     if (warp >= kEpi && warp < kMma) {
         // ------------------------------ x / e -> shared memory ------------------------------
         // a warp takes the 16-byte columns w, w + 4 of every piece; x and e have the same type in the backward
-        const int w = warp - kEpi;
+        const int w = (warp - kEpi) & 3, group = (warp - kEpi) >> 2;
         constexpr int NI = KC / 32;                       // items a thread has in a piece
         const int total = (pl.reuse ? my : jobs) * nA;
-        auto load = [&](Item<IN>(&it)[NI], int a) {
-            const int kc = a % nA;
-            const uint32_t n0 = tile_at(a / nA / (pl.reuse ? 1 : pl.nJ)) * TP;
-            const bool is_x = !BWD || kc < pl.nKx;
+        // The group's place in the sequence of pieces (tile k, chunk j, piece kc), for the loads and for the stores,
+        // which run one piece behind; the slot and its phase go with the stores.
+        struct Place {
+            int k, j, kc;
+        };
+        const int chunks = pl.reuse ? 1 : pl.nJ;
+        auto advance = [&](Place& q) {
+            for (q.kc += kGroups; q.kc >= nA;) {
+                q.kc -= nA;
+                if (++q.j == chunks) {
+                    q.j = 0;
+                    ++q.k;
+                }
+            }
+        };
+        auto load = [&](Item<IN>(&it)[NI], Place& q) {
+            if (q.k >= my) return;
+            const bool is_x = !BWD || q.kc < pl.nKx;
             const IN* src = static_cast<const IN*>(is_x ? p.x : p.gy);
-            const int k0 = (is_x ? kc : kc - pl.nKx) * KC;
+            const int k0 = (is_x ? q.kc : q.kc - pl.nKx) * KC;
 #pragma unroll
             for (int i = 0; i < NI; ++i)
-                load_item<IN>(it[i], src, is_x ? pl.C : pl.O, k0 + (w + 4 * i) * 8, n0, lane, p);
+                load_item<IN>(it[i], src, is_x ? pl.C : pl.O, k0 + (w + 4 * i) * 8, tile_at(q.k) * TP, lane, p);
+            advance(q);
         };
-        auto put = [&](const Item<IN>(&it)[NI], int a) -> bool {
-            const int kc = a % nA, slot = a % pl.na, use = a / pl.na;
-            const int pw = !BWD || kc < pl.nKx ? piece_k(pl.Kx, KC, kc) : piece_k(pl.Ky, KC, kc - pl.nKx);
-            if (use > 0 && !wait(&bar.empty_a[slot], (uint32_t)(use - 1) & 1)) return false;
+        int slot = group % pl.na;
+        uint32_t phase = 1 ^ ((group / pl.na) & 1);       // of the slot's last release: none is needed the first time
+        auto put = [&](const Item<IN>(&it)[NI], Place& q) -> bool {
+            if (q.k >= my) return false;
+            const bool is_x = !BWD || q.kc < pl.nKx;
+            const int pw = is_x ? piece_k(pl.Kx, KC, q.kc) : piece_k(pl.Ky, KC, q.kc - pl.nKx);
+            if (!wait(&bar.empty_a[slot], phase)) return false;  // (a new barrier's phase before the first is complete)
             char* s = sm + pl.o_a + slot * pl.a_slot;
 #pragma unroll
             for (int i = 0; i < NI; ++i)
                 if ((w + 4 * i) * 8 < pw) store_item<T, IN>(it[i], s, w + 4 * i, pw / 16, lane, p.vec);
             if constexpr (BWD) {  // x and e go to the scratch too, once a tile
-                const int k = a / nA;
-                if (p.z && (pl.reuse || k % pl.nJ == 0)) {
-                    const bool is_x = kc < pl.nKx;
-                    const int c0 = (is_x ? kc : kc - pl.nKx) * KC, rows = is_x ? pl.C : pl.O;
-                    const int tile = (pl.reuse ? k : k / pl.nJ) * (int)gridDim.x + (int)blockIdx.x;
+                if (p.z && p.z_rows > 3 * pl.H && q.j == 0) {
+                    const int c0 = (is_x ? q.kc : q.kc - pl.nKx) * KC, rows = is_x ? pl.C : pl.O;
                     T* z = static_cast<T*>(p.z) +
-                           ((int64_t)tile * (3 * pl.H + pl.C + pl.O) + 3 * pl.H + (is_x ? 0 : pl.C)) * TP;
+                           ((int64_t)(tile_at(q.k) - p.tile0) * p.z_rows + 3 * pl.H + (is_x ? 0 : pl.C)) * TP;
 #pragma unroll
                     for (int i = 0; i < NI; ++i) copy_item<T>(it[i], z, c0 + (w + 4 * i) * 8, rows, lane, p.vec);
                 }
@@ -583,17 +642,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&bar.full_a[slot]);
+            for (slot += kGroups; slot >= pl.na;) {
+                slot -= pl.na;
+                phase ^= 1;
+            }
+            advance(q);
             return true;
         };
-        // the next piece's loads are in flight while this one waits for its slot and is written
+        // the group's next piece is in flight while this one waits for its slot and is written
         Item<IN> c[NI], d[NI];
-        if (total > 0) load(c, 0);
-        for (int a = 0; a < total; a += 2) {
-            if (a + 1 < total) load(d, a + 1);
-            if (!put(c, a)) break;
-            if (a + 1 >= total) break;
-            if (a + 2 < total) load(c, a + 2);
-            if (!put(d, a + 1)) break;
+        Place in{0, 0, group - kGroups}, at;
+        advance(in);
+        at = in;
+        load(c, in);
+        while (true) {
+            load(d, in);
+            if (!put(c, at)) break;
+            load(c, in);
+            if (!put(d, at)) break;
         }
     } else if (warp == kLoad) {
         // ------------------------------ weights -> shared memory ------------------------------
@@ -741,7 +807,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                 }
                 if (J > 0) {  // second product of job J - 1
                     if (!all(&bar.mid[b ^ 1], (uint32_t)((J - 1) >> 1) & 1)) break;
-                    if (j2 == 0 && k2 > 0 && !all(&bar.d2_free, (uint32_t)(k2 - 1) & 1)) break;
+                    const int e = d2_buf(k2);
+                    if (j2 == 0 && d2_use(k2) > 0 && !all(&bar.d2_free[e], (uint32_t)(d2_use(k2) - 1) & 1)) break;
+                    const uint32_t d2 = d2_0 + e * d2w;
                     fence_after();
                     const uint32_t d = tmem + (b ^ 1) * d1w;
                     int at = j2 * pl.job_bytes + pl.NH * (2 * pl.Kx + pl.Ky) * 2 * SPL;
@@ -768,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                     if (!ok) break;
                     commit(&bar.g2[b ^ 1], leader);
                     if (++j2 == pl.nJ) {
-                        commit(&bar.d2, leader);
+                        commit(&bar.d2[e], leader);
                         j2 = 0;
                         ++k2;
                     }
@@ -779,30 +847,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
             tc::mbar_wait(&bar.drain, 0, nullptr);
         }
     } else if (warp < kEpi) {
-        // ------------------------------ middle and output ------------------------------
-        const int quad = warp & 3, half = warp >> 2;      // lane quadrant; which 16-column groups
+        // ------------------------------ middle ------------------------------
+        const int quad = warp & 3, part = warp >> 2;      // lane quadrant; which 16-column groups
         const int row = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const int groups = pl.NH / 16;
 
-        auto middle = [&](int J) -> bool {
-            const int b = J & 1, j = J % pl.nJ;
-            const uint32_t tile = tile_at(J / pl.nJ), n = tile * TP + row;
+        auto middle = [&](int J, int k, int j) -> bool {
+            const int b = J & 1;
+            const uint32_t tile = tile_at(k), n = tile * TP + row;
             const bool valid = n < p.points;
             float sc = 1.f;
             if constexpr (sizeof(IN) == 1) sc = valid ? __ldg(p.scale + n) : 0.f;
             if (!wait(&bar.d1[b], (uint32_t)(J >> 1) & 1)) return false;
             fence_after();
             const uint32_t d = tmem + b * d1w + lanes;
-            for (int g = half; g < groups; g += 2) {
+            for (int g = part; g < groups; g += kEpi / 4) {
                 float vg[16], vu[16];
                 ld16(d + 16 * g, vg);
                 ld16(d + pl.NH + 16 * g, vu);
+                const int h0 = j * pl.NH + 16 * g;
+                float4 bg[4], bu[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    bg[i] = reinterpret_cast<const float4*>(bias_g + h0)[i];
+                    bu[i] = reinterpret_cast<const float4*>(bias_u + h0)[i];
+                }
                 wait_ld(vg);
                 wait_ld(vu);
-                const int h0 = j * pl.NH + 16 * g;
-                const float4* bg = reinterpret_cast<const float4*>(bias_g + h0);
-                const float4* bu = reinterpret_cast<const float4*>(bias_u + h0);
                 float2 g2[8], u2[8];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -831,9 +903,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                     float vf[16];
                     ld16(d + 2 * pl.NH + 16 * g, vf);
                     wait_ld(vf);
-                    T* z = static_cast<T*>(p.z) + ((int64_t)(tile - p.tile0) * (3 * pl.H + pl.C + pl.O) + h0) * TP + row;
+                    T* z = static_cast<T*>(p.z) + ((int64_t)(tile - p.tile0) * p.z_rows + h0) * TP + row;
                     T *zu = z + pl.H * TP, *zh = zu + pl.H * TP;
                     const int left = p.z ? pl.H - h0 : 0;
+                    uint32_t w[2][SPL][8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         float2 slope;
@@ -841,29 +914,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                         // points past the last one are zeros in the scratch
                         const float2 f = valid ? make_float2(vf[2 * i], vf[2 * i + 1]) : both(0.f);
                         const float2 h = valid ? __fmul2_rn(a, u2[i]) : both(0.f);
-                        g2[i] = __fmul2_rn(__fmul2_rn(f, u2[i]), slope);
-                        u2[i] = __fmul2_rn(f, a);
-                        if (2 * i < left) {
-                            z[2 * i * TP] = from_f<T>(g2[i].x);
-                            zu[2 * i * TP] = from_f<T>(u2[i].x);
-                            zh[2 * i * TP] = from_f<T>(h.x);
-                        }
-                        if (2 * i + 1 < left) {
-                            z[(2 * i + 1) * TP] = from_f<T>(g2[i].y);
-                            zu[(2 * i + 1) * TP] = from_f<T>(u2[i].y);
-                            zh[(2 * i + 1) * TP] = from_f<T>(h.y);
-                        }
-                    }
-                    uint32_t w[2][SPL][8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                        const float2 dg = __fmul2_rn(__fmul2_rn(f, u2[i]), slope), du = __fmul2_rn(f, a);
                         uint32_t t[SPL], r[SPL];
-                        images<T>(g2[i], t);
-                        images<T>(u2[i], r);
+                        images<T>(dg, t);
+                        images<T>(du, r);
 #pragma unroll
                         for (int s = 0; s < SPL; ++s) {
                             w[0][s][i] = t[s];
                             w[1][s][i] = r[s];
+                        }
+                        if constexpr (SPL == 1) {
+                            uint32_t o[1];
+                            images<T>(h, o);
+                            store_rows(z + 2 * i * TP, t[0], lane, left - 2 * i);
+                            store_rows(zu + 2 * i * TP, r[0], lane, left - 2 * i);
+                            store_rows(zh + 2 * i * TP, o[0], lane, left - 2 * i);
+                        } else {
+                            if (2 * i < left) {
+                                z[2 * i * TP] = dg.x;
+                                zu[2 * i * TP] = du.x;
+                                zh[2 * i * TP] = h.x;
+                            }
+                            if (2 * i + 1 < left) {
+                                z[(2 * i + 1) * TP] = dg.y;
+                                zu[(2 * i + 1) * TP] = du.y;
+                                zh[(2 * i + 1) * TP] = h.y;
+                            }
                         }
                     }
                     if constexpr (SPL == 1) {
@@ -889,11 +965,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
             const uint32_t n = tile_at(k) * TP + row;
             const bool valid = n < p.points;
             const int width = BWD ? pl.C : pl.O;      // the field's channels
-            const uint32_t b = valid ? n / p.P : 0;
+            const uint32_t b = valid ? sample_of(p, n) : 0;
             T* y = static_cast<T*>(p.out) + ((int64_t)b * width + pl.col0) * p.P + (valid ? n - b * p.P : 0);
-            if (!wait(&bar.d2, (uint32_t)k & 1)) return false;
+            const int e = d2_buf(k);
+            if (!wait(&bar.d2[e], (uint32_t)d2_use(k) & 1)) return false;
             fence_after();
-            for (int g = half; g < pl.N2 / 16; g += 2) {
+            const uint32_t d2 = d2_0 + e * d2w;
+            const int n16 = pl.N2 / 16;
+            if (part >= n16) {  // a warp without columns
+                fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bar.d2_free[e]);
+            }
+            for (int g = part; g < n16; g += kEpi / 4) {
                 float v[16];
                 ld16(d2 + lanes + 16 * g, v);
                 wait_ld(v);
@@ -903,6 +987,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                     wait_ld(c);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] += c[i];
+                }
+                if (g + kEpi / 4 >= n16) {  // read: the next second product may begin while this goes out
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&bar.d2_free[e]);
                 }
                 if constexpr (!BWD) {  // all loads before the stores, which might alias them for all the compiler knows
                     const float4* b2 = reinterpret_cast<const float4*>(bias_2 + 16 * g);
@@ -927,15 +1016,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
                         if (i < left) yg[(int64_t)i * p.P] = from_f<T>(v[i]);
                 }
             }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&bar.d2_free);
             return true;
         };
         bool ok = true;
-        for (int J = 0; J < jobs && ok; ++J) {
-            ok = middle(J);
-            if (ok && J > 0 && J % pl.nJ == 0) ok = output(J / pl.nJ - 1);
+        for (int J = 0, k = 0; k < my && ok; ++k) {
+            for (int j = 0; j < pl.nJ && ok; ++j, ++J) {
+                ok = middle(J, k, j);
+                if (ok && j == 0 && k > 0) ok = output(k - 1);
+            }
         }
         if (ok && my > 0) output(my - 1);
     }
@@ -948,15 +1036,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const __grid_constant__ P
 // ------------------------------------------------------------------------------------------------
 // weight gradients
 // ------------------------------------------------------------------------------------------------
-constexpr int kWork = 4;                      // warps 8..11: fp32 splitting, row sums (warps 0..7: accumulators)
-constexpr int kWMma = 8 + kWork, kWLoad = kWMma + 1;
-constexpr int kWThreads = 32 * (kWLoad + 1);
 constexpr int kPromote = 8;                   // pieces an accumulator runs before it goes to registers
 constexpr int kImages = 2;                    // fp32: stages of split operands
 
 // A piece is 128 bytes of points of up to 128 rows of each operand, as a 128-byte-swizzled tensor copy leaves them:
 // for 16-bit types that is the MMA's own K-major layout and the pieces are multiplied as they land.
 template <class T> struct WForm {
+    // warps 0..7: accumulators; then fp32 splitting (four warps an operand) and row sums, MMA issue, copies
+    static constexpr int WORK = sizeof(T) == 4 ? 8 : 4, MMA = 8 + WORK, LOAD = MMA + 1, THREADS = 32 * (LOAD + 1);
     static constexpr int KC = 128 / (int)sizeof(T);
     static constexpr int STAGES = sizeof(T) == 4 ? 3 : 6;
     static constexpr int RAW = 2 * 128 * 128;                        // A rows, then B rows
@@ -970,6 +1057,7 @@ struct WParams {
     double* sums;              // [split][2 H + O] row sums of dg, du and e (may be NULL)
     int C, H, O;
     int rows;                  // rows of a tile of the scratch
+    int tile0, per_sample;     // x and e in place: the slab's first tile, tiles of a sample; per_sample 0: in the scratch
     int pieces;                // pieces of KC points in the slab
     int splits;
     int nC, nO;                // column tiles of x and of e
@@ -990,9 +1078,9 @@ __device__ __forceinline__ uint64_t desc_128b(uint32_t addr) {  // K-major rows 
 // CTA = (tile, split).  Tile: 128 rows of the scratch (rows of [dg; du] against rows of x, rows of h against rows of
 // e) x up to 128 columns; K: the split's share of the slab's points.
 template <class T>
-__global__ void __launch_bounds__(kWThreads, 1)
-k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mx,
-        const __grid_constant__ CUtensorMap me, const __grid_constant__ WParams p, int* __restrict__ status) {
+__global__ void __launch_bounds__(WForm<T>::THREADS, 1)
+k_wgrad(const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensorMap mh,
+        const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap me, const __grid_constant__ WParams p, int* __restrict__ status) {
     using W = WForm<T>;
     constexpr int SPL = Form<T>::SPL, KC = W::KC, NP = Passes<SPL>::N, S = W::STAGES;
     constexpr bool kSplit = SPL > 1;
@@ -1016,10 +1104,10 @@ k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
     if (tid == 0) {
         for (int i = 0; i < S; ++i) {
             tc::mbar_init(&bar.raw[i], 1);
-            tc::mbar_init(&bar.raw_free[i], kSplit ? kWork : working ? kWork + 1 : 1);
+            tc::mbar_init(&bar.raw_free[i], kSplit ? W::WORK : working ? W::WORK + 1 : 1);
         }
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(&bar.img[i], kWork);
+            tc::mbar_init(&bar.img[i], W::WORK);
             tc::mbar_init(&bar.img_free[i], 1);
             tc::mbar_init(&bar.acc[i], 1);
             tc::mbar_init(&bar.acc_free[i], 8);
@@ -1039,19 +1127,21 @@ k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
     fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, bar.tmem, 0);
     auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
-        if (tc::mbar_wait(b, parity, abort_flag)) return true;
+        if (wait_for(b, parity, abort_flag)) return true;
         *abort_flag = 1;
         atomicExch(status, tc::kStatusMmaTimeout);
         return false;
     };
     char* split_at = sm + S * W::RAW;
 
-    if (warp == kWLoad) {
+    if (warp == W::LOAD) {
         // ------------------------------ scratch -> shared memory ------------------------------
         if (lane == 0) {
             const CUtensorMap* mb = of_x ? &mx : &me;
-            const int a0 = (of_x ? 0 : 2 * p.H) + mt * 128, b0 = 3 * p.H + (of_x ? 0 : p.C) + nt * 128;
-            const uint32_t bytes = (uint32_t)(128 + imin(128, of_x ? p.C : p.O)) * 128;
+            const int a0 = (of_x ? 0 : 2 * p.H) + mt * 128;
+            const int b0 = nt * 128 + (p.per_sample ? 0 : 3 * p.H + (of_x ? 0 : p.C));
+            const CUtensorMap* ma = of_x ? &mg : &mh;
+            const uint32_t bytes = (uint32_t)(imin(128, of_x ? 2 * p.H : p.H) + imin(128, of_x ? p.C : p.O)) * 128;
             int k = 0;
             for (; k < steps; ++k) {
                 const int slot = k % S, use = k / S;
@@ -1061,22 +1151,28 @@ k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(&bar.raw[slot])),
                              "r"(bytes)
                              : "memory");
-                auto copy = [&](uint32_t to, const CUtensorMap* m, int row) {
+                auto copy = [&](uint32_t to, const CUtensorMap* m, int c, int row) {
                     asm volatile(
                         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
                         "%3}], [%4];" ::"r"(to),
                         "l"(reinterpret_cast<uint64_t>(m)), "r"(c), "r"(row), "r"(tc::smem_u32(&bar.raw[slot]))
                         : "memory");
                 };
-                copy(dst, &ma, t * p.rows + a0);
-                copy(dst + W::RAW / 2, mb, t * p.rows + b0);
+                copy(dst, ma, c, t * p.rows + a0);
+                if (p.per_sample) {
+                    const int s = (p.tile0 + t) / p.per_sample, first = (p.tile0 + t - s * p.per_sample) * TP;
+                    copy(dst + W::RAW / 2, mb, first + c, s * (of_x ? p.C : p.O) + b0);
+                } else {
+                    copy(dst + W::RAW / 2, mb, c, t * p.rows + b0);
+                }
             }
             for (int i = 0; i < S && i < k; ++i)  // no copy outlives the CTA (bounded)
                 tc::mbar_wait(&bar.raw[(k - 1 - i) % S], (uint32_t)((k - 1 - i) / S) & 1, nullptr);
         }
-    } else if (warp >= 8 && warp < kWMma) {
+    } else if (warp >= 8 && warp < W::MMA) {
         // ------------------------------ splitting and row sums: a thread has a row of each operand ----------------
-        const int r = tid - 256;
+        const int r = (tid - 256) & 127, o = kSplit ? (tid - 256) >> 7 : want_b;  // row, operand
+        const bool summing = o ? want_b : want_a;
         double sum = 0.0;
         auto row_of = [&](const char* raw, float (&v)[KC]) {
             const char* row = raw + r * 128;
@@ -1102,9 +1198,7 @@ k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
             if constexpr (kSplit) {
                 const int si = k % kImages, use = k / kImages;
                 if (use > 0 && !wait(&bar.img_free[si], (uint32_t)(use - 1) & 1)) break;
-#pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    if (o && r >= n) break;
+                if (!o || r < n) {
                     row_of(raw + o * (W::RAW / 2), v);
                     char* to = split_at + si * W::SPLIT + o * SPL * W::IMG + (r >> 3) * 256 + (r & 7) * 16;
 #pragma unroll
@@ -1117,10 +1211,10 @@ k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
                             *reinterpret_cast<uint4*>(to + q * W::IMG + (ch >> 1) * (128 * 32) + (ch & 1) * 128) =
                                 make_uint4(img[0][q], img[1][q], img[2][q], img[3][q]);
                     }
-                    if (o ? want_b : want_a) add(v);
+                    if (summing) add(v);
                 }
             } else {
-                row_of(raw + (want_b ? W::RAW / 2 : 0), v);
+                row_of(raw + o * (W::RAW / 2), v);
                 add(v);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1130,11 +1224,11 @@ k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
                 tc::mbar_arrive(&bar.raw_free[slot]);
             }
         }
-        if ((want_a && r < a_rows) || (want_b && r < b_rows)) {
-            double* out = p.sums + (int64_t)split * (2 * p.H + p.O) + (want_a ? mt * 128 : 2 * p.H + nt * 128) + r;
+        if (summing && r < (o ? b_rows : a_rows)) {
+            double* out = p.sums + (int64_t)split * (2 * p.H + p.O) + (o ? 2 * p.H + nt * 128 : mt * 128) + r;
             *out = p.accumulate ? *out + sum : sum;
         }
-    } else if (warp == kWMma) {
+    } else if (warp == W::MMA) {
         // ------------------------------ MMA issue ------------------------------
         const uint32_t leader = elect_one();
         const uint32_t id = idesc_of(Form<T>::kFmt, n);
@@ -1204,19 +1298,21 @@ k_wgrad(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 if ((half + 2 * g) * 16 < n) {
-                    float v[16];
                     const uint32_t at = tmem + buf * DW + (half + 2 * g) * 16 + ((uint32_t)(quad * 32) << 16);
-                    ld16(at, v);
-                    wait_ld(v);
-                    if constexpr (SPL == 3) {
-                        float c[16];
-                        ld16(at + 128, c);
-                        wait_ld(c);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] += c[i];
+                    for (int i = 0; i < 16; i += 8) {
+                        float v[8], c[8] = {};
+                        tc::tmem_ld8(at + i, v);
+                        if (kSplit) tc::tmem_ld8(at + 128 + i, c);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                                     : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                                       "+f"(v[7]), "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]), "+f"(c[4]), "+f"(c[5]),
+                                       "+f"(c[6]), "+f"(c[7])
+                                     :
+                                     : "memory");
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sum[g][i + e] += kSplit ? v[e] + c[e] : v[e];
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[g][i] += v[i];
                 }
             }
             fence_before();
@@ -1287,8 +1383,9 @@ k_finish(WParams p, T* __restrict__ gwg, T* __restrict__ gwu, T* __restrict__ gw
 // ------------------------------------------------------------------------------------------------
 // How a call is cut.  An fp32 launch takes at most 128 output channels (D2 and D2c); more are several launches, each
 // with the whole first product.  Tensor memory: two D1 buffers and D2 (fp32: and D2c) in 512 columns, so the
-// backward's chunk (three columns a hidden channel) is 64 wide when D2 takes up to 128 of them and 32 above.  Shared memory: the weights stay when they
-// leave room for two pieces of A, otherwise two to four pieces of each stream.
+// backward's chunk (three columns a hidden channel) is 64 wide when D2 takes up to 128 of them and 32 above; what is
+// left may hold a second D2.  Shared memory: the weights stay when they
+// leave room for two pieces of A, otherwise two to six pieces of each stream.
 template <class T>
 bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
     constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC;
@@ -1304,6 +1401,7 @@ bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
     const int most = bwd && p.N2 * (SPL == 3 ? 2 : 1) > 128 ? 32 : 64;
     p.nJ = (p.H + most - 1) / most;
     p.NH = up16((p.H + p.nJ - 1) / p.nJ);
+    p.n_d2 = 2 * (bwd ? 3 : 2) * p.NH + 2 * p.N2 * (SPL == 3 ? 2 : 1) <= 512 ? 2 : 1;
     p.nKx = (p.Kx + KC - 1) / KC;
     p.nKy = (p.Ky + KC - 1) / KC;
     p.nH = (p.NH + KC - 1) / KC;
@@ -1328,7 +1426,7 @@ bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
         // spare room: first for as many A pieces as a tile has, then for weights
         p.na = 2;
         while (p.na < kMaxA && p.na < nA && (p.na + 1) * p.a_slot + 2 * (int64_t)p.b_slot <= room) ++p.na;
-        while (p.nb < 4 && p.na * p.a_slot + (p.nb + 1) * (int64_t)p.b_slot <= room) ++p.nb;
+        while (p.nb < 6 && p.na * p.a_slot + (p.nb + 1) * (int64_t)p.b_slot <= room) ++p.nb;
         while (p.na < kMaxA && (p.na + 1) * p.a_slot + p.nb * (int64_t)p.b_slot <= room) ++p.na;
         bytes = (int64_t)p.nb * p.b_slot;
     }
@@ -1439,13 +1537,13 @@ typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, v
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// rows of 128 points, boxes of 128 bytes x `box` rows
+// `rows` rows of `points` points, boxes of 128 bytes x `box` rows
 template <class T>
-bool row_map(CUtensorMap* m, void* base, int64_t rows, int box) {
+bool row_map(CUtensorMap* m, void* base, int64_t points, int64_t rows, int box) {
     const EncodeTiled enc = reinterpret_cast<EncodeTiled>(tensor_map_encoder());
     if (!enc) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)TP, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)TP * sizeof(T)};
+    const cuuint64_t dims[2] = {(cuuint64_t)points, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)points * sizeof(T)};
     const cuuint32_t sizes[2] = {(cuuint32_t)(128 / sizeof(T)), (cuuint32_t)box};
     const cuuint32_t ones[2] = {1, 1};
     const CUtensorMapDataType type = std::is_same<T, float>::value    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
@@ -1482,6 +1580,10 @@ Params params_of(const nop_gated_desc& d, const Plan& p, const nop_gated_operand
     q.bias = reinterpret_cast<const float*>(ws + z.vec);
     q.P = (uint32_t)d.points;
     q.points = (uint32_t)(d.batch * d.points);
+    uint32_t s = 0;
+    while ((1ull << s) < d.points) ++s;
+    q.p_shift = 31 + s;
+    q.p_mul = (uint32_t)(((1ull << q.p_shift) + d.points - 1) / d.points);
     q.tiles = (int)z.tiles;
     q.pl = p;
     return q;
@@ -1499,8 +1601,8 @@ int32_t forward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, co
         q.out = o.y;
         q.vec = d.points % 4 == 0 && aligned({o.x}, 4 * sizeof(IN));
         rc = d.activation == NOP_ACT_GELU
-                 ? launch(k_block<T, IN, false, true>, grid, kThreads, p.smem, s, q, dev.status)
-                 : launch(k_block<T, IN, false, false>, grid, kThreads, p.smem, s, q, dev.status);
+                 ? launch(k_block<T, IN, false, true>, grid, Roles<false>::THREADS, p.smem, s, q, dev.status)
+                 : launch(k_block<T, IN, false, false>, grid, Roles<false>::THREADS, p.smem, s, q, dev.status);
         if (rc != NOP_OK || p.col0 + p.cols >= p.O) return rc;
         if (!make_plan<T>(d, false, p.col0 + p.cols, &p)) return fail(NOP_E_UNSUPPORTED, kTooLarge);
     }
@@ -1525,18 +1627,28 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
     w.C = p.C;
     w.H = p.H;
     w.O = p.O;
-    w.rows = 3 * p.H + p.C + p.O;
+    // x and e in place: whole tiles a sample, on 16-byte boundaries
+    const bool in_place = d.points % TP == 0 && aligned({o.x, g.gy}, 16);
+    w.rows = 3 * p.H + (in_place ? 0 : p.C + p.O);
+    w.per_sample = in_place ? (int)(d.points / TP) : 0;
+    q.z_rows = w.rows;
     w.nC = (int)ceil_div(p.C, 128);
     w.nO = (int)ceil_div(p.O, 128);
     w.mX = (int)ceil_div(2 * p.H, 128);
     w.mH = (int)ceil_div(p.H, 128);
     w.splits = z.splits;
-    CUtensorMap ma{}, mx{}, me{};
+    CUtensorMap mg{}, mh{}, mx{}, me{};
     if (weights) {
         const int64_t rows = z.slab_tiles * w.rows;
-        if (!row_map<T>(&ma, ws + z.z, rows, 128) || !row_map<T>(&mx, ws + z.z, rows, imin(128, p.C)) ||
-            !row_map<T>(&me, ws + z.z, rows, imin(128, p.O)))
-            return fail(NOP_E_CUDA, "cuTensorMapEncodeTiled(scratch) failed");
+        void *xs = ws + z.z, *es = ws + z.z;
+        if (in_place) {
+            xs = const_cast<void*>(o.x);
+            es = const_cast<void*>(g.gy);
+        }
+        if (!row_map<T>(&mg, ws + z.z, TP, rows, imin(128, 2 * p.H)) || !row_map<T>(&mh, ws + z.z, TP, rows, imin(128, p.H)) ||
+            !row_map<T>(&mx, xs, in_place ? d.points : TP, in_place ? d.batch * p.C : rows, imin(128, p.C)) ||
+            !row_map<T>(&me, es, in_place ? d.points : TP, in_place ? d.batch * p.O : rows, imin(128, p.O)))
+            return fail(NOP_E_CUDA, "cuTensorMapEncodeTiled failed");
     }
     const int64_t slab = weights ? z.slab_tiles : z.tiles;
     constexpr int wsmem = WForm<T>::BODY + (int)sizeof(WBars);
@@ -1544,13 +1656,14 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
         q.tile0 = (int)t;
         q.tiles = (int)std::min<int64_t>(slab, z.tiles - t);
         const unsigned grid = (unsigned)std::min<int64_t>(q.tiles, dev.sms);
-        rc = d.activation == NOP_ACT_GELU ? launch(k_block<T, T, true, true>, grid, kThreads, p.smem, s, q, dev.status)
-                                          : launch(k_block<T, T, true, false>, grid, kThreads, p.smem, s, q, dev.status);
+        rc = d.activation == NOP_ACT_GELU ? launch(k_block<T, T, true, true>, grid, Roles<true>::THREADS, p.smem, s, q, dev.status)
+                                          : launch(k_block<T, T, true, false>, grid, Roles<true>::THREADS, p.smem, s, q, dev.status);
         if (rc != NOP_OK) return rc;
         if (!weights) continue;
         w.pieces = q.tiles * (TP / WForm<T>::KC);
+        w.tile0 = (int)t;
         w.accumulate = t > 0;
-        rc = launch(k_wgrad<T>, (unsigned)(z.splits * z.wtiles), kWThreads, wsmem, s, ma, mx, me, w, dev.status);
+        rc = launch(k_wgrad<T>, (unsigned)(z.splits * z.wtiles), WForm<T>::THREADS, wsmem, s, mg, mh, mx, me, w, dev.status);
         if (rc != NOP_OK) return rc;
     }
     // dL/dx of the channels past the first launch's: the products again, without the scratch
@@ -1562,8 +1675,8 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
         r.out = q.out;
         r.vec = q.vec;
         const unsigned grid = (unsigned)std::min<int64_t>(z.tiles, dev.sms);
-        rc = d.activation == NOP_ACT_GELU ? launch(k_block<T, T, true, true>, grid, kThreads, p.smem, s, r, dev.status)
-                                          : launch(k_block<T, T, true, false>, grid, kThreads, p.smem, s, r, dev.status);
+        rc = d.activation == NOP_ACT_GELU ? launch(k_block<T, T, true, true>, grid, Roles<true>::THREADS, p.smem, s, r, dev.status)
+                                          : launch(k_block<T, T, true, false>, grid, Roles<true>::THREADS, p.smem, s, r, dev.status);
         if (rc != NOP_OK) return rc;
     }
     if (!weights) return NOP_OK;
