@@ -392,41 +392,22 @@ template <class IN> struct Item {
     uint32_t w[8 * W];
 };
 
-// lane's 4 points: 4 lane .. 4 lane + 3 of the tile (vec), or lane, lane + 32, ... (any alignment)
+// A lane's 4 points are 4 lane .. 4 lane + 3 of the tile, but lane, lane + 32, ... of an fp32 field whose rows are
+// not aligned (its single loads are then a line each).
+template <class IN> __device__ __forceinline__ bool neighbours(bool vec) { return vec || sizeof(IN) < 4; }
+
+// The 4 points one by one, whatever their samples; into r as an Item's words
 template <class IN>
-__device__ __forceinline__ void load_item(Item<IN>& it, const IN* __restrict__ src, int C, int c0, uint32_t n0, int lane,
-                                          const Params& p) {
+__device__ __forceinline__ void load_singly(uint32_t* r, int stride, const IN* __restrict__ src, int C, int c0,
+                                            uint32_t n0, int lane, const Params& p) {
     constexpr int W = Item<IN>::W;
-    if (p.vec) {
-        const uint32_t n = n0 + 4 * lane;
-        const bool ok = n < p.points;
-        const uint32_t b = ok ? sample_of(p, n) : 0;
-        const IN* s = src + (int64_t)b * C * p.P + (ok ? n - b * p.P : 0) + (int64_t)c0 * p.P;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const bool in = ok && c0 + e < C;
-            const IN* a = s + (int64_t)e * p.P;
-            if constexpr (W == 4) {
-                const uint4 q = in ? __ldg(reinterpret_cast<const uint4*>(a)) : make_uint4(0, 0, 0, 0);
-                it.w[4 * e] = q.x;
-                it.w[4 * e + 1] = q.y;
-                it.w[4 * e + 2] = q.z;
-                it.w[4 * e + 3] = q.w;
-            } else if constexpr (W == 2) {
-                const uint2 q = in ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
-                it.w[2 * e] = q.x;
-                it.w[2 * e + 1] = q.y;
-            } else {
-                it.w[e] = in ? __ldg(reinterpret_cast<const uint32_t*>(a)) : 0;
-            }
-        }
-        return;
-    }
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int e = 0; e < 8 * W; ++e) it.w[e] = 0;
+        for (int i = 0; i < W; ++i) r[e * stride + i] = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t n = n0 + lane + 32 * i;
+        const uint32_t n = n0 + (W < 4 ? 4 * lane + i : lane + 32 * i);
         if (n >= p.points) continue;
         const uint32_t b = sample_of(p, n);
         const IN* s = src + (int64_t)b * C * p.P + (n - b * p.P) + (int64_t)c0 * p.P;
@@ -434,11 +415,99 @@ __device__ __forceinline__ void load_item(Item<IN>& it, const IN* __restrict__ s
         for (int e = 0; e < 8; ++e) {
             if (c0 + e >= C) continue;
             const IN* a = s + (int64_t)e * p.P;
-            if constexpr (W == 4) it.w[4 * e + i] = __ldg(reinterpret_cast<const uint32_t*>(a));
+            if constexpr (W == 4) r[e * stride + i] = __ldg(reinterpret_cast<const uint32_t*>(a));
             else if constexpr (W == 2)
-                it.w[2 * e + i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(a)) << (16 * (i & 1));
+                r[e * stride + i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(a)) << (16 * (i & 1));
             else
-                it.w[e] |= (uint32_t)__ldg(reinterpret_cast<const uint8_t*>(a)) << (8 * i);
+                r[e * stride] |= (uint32_t)__ldg(reinterpret_cast<const uint8_t*>(a)) << (8 * i);
+        }
+    }
+}
+
+template <class IN>
+__device__ __forceinline__ void load_item(uint32_t* r, const IN* __restrict__ src, int C, int c0, uint32_t n0, int lane,
+                                          const Params& p) {
+    constexpr int W = Item<IN>::W;
+    if (!p.vec) {
+        load_singly<IN>(r, W, src, C, c0, n0, lane, p);
+        return;
+    }
+    const uint32_t n = n0 + 4 * lane;
+    const bool ok = n < p.points;
+    const uint32_t b = ok ? sample_of(p, n) : 0;
+    const IN* s = src + (int64_t)b * C * p.P + (ok ? n - b * p.P : 0) + (int64_t)c0 * p.P;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const bool in = ok && c0 + e < C;
+        const IN* a = s + (int64_t)e * p.P;
+        if constexpr (W == 4) {
+            const uint4 q = in ? __ldg(reinterpret_cast<const uint4*>(a)) : make_uint4(0, 0, 0, 0);
+            r[4 * e] = q.x;
+            r[4 * e + 1] = q.y;
+            r[4 * e + 2] = q.z;
+            r[4 * e + 3] = q.w;
+        } else if constexpr (W == 2) {
+            const uint2 q = in ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
+            r[2 * e] = q.x;
+            r[2 * e + 1] = q.y;
+        } else {
+            r[e] = in ? __ldg(reinterpret_cast<const uint32_t*>(a)) : 0;
+        }
+    }
+}
+
+// A narrow field on rows of any alignment: a channel's 4 values lie in two aligned words of 4 values, which are loaded
+// as they are and cut when the item is used (cut_item) -- combined here, they would make the producer wait for every
+// load.  Returns the first channel's offset in its word, or 8 where the words would leave the field or the points are
+// not of one sample, and the values have been loaded one by one.
+template <class IN>
+__device__ __forceinline__ uint32_t load_around(uint32_t* r, const IN* __restrict__ src, int C, int c0, uint32_t n0,
+                                                int lane, const Params& p) {
+    constexpr int W = Item<IN>::W, N = 4 * W;
+    const uint32_t n = n0 + 4 * lane;
+    const uint32_t b = n < p.points ? sample_of(p, n) : 0, o = n - b * p.P;
+    const char* first = reinterpret_cast<const char*>(src + (int64_t)b * C * p.P + o + (int64_t)c0 * p.P);
+    const char *begin = reinterpret_cast<const char*>(src), *end = begin + (int64_t)p.points * C * W;
+    auto word = [&](int e) {
+        return reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(first + (int64_t)e * p.P * W) & ~(uintptr_t)(N - 1));
+    };
+    const int last = imin(8, C - c0) - 1;
+    if (last < 0 || n + 3 >= p.points || o + 3 >= p.P || word(0) < begin || word(last) + 2 * N > end) {
+        load_singly<IN>(r, 2 * W, src, C, c0, n0, lane, p);
+        return 8;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (W == 2) {
+            const uint2* a = reinterpret_cast<const uint2*>(word(e));
+            const uint2 q = e <= last ? __ldg(a) : make_uint2(0, 0), t = e <= last ? __ldg(a + 1) : make_uint2(0, 0);
+            r[4 * e] = q.x;
+            r[4 * e + 1] = q.y;
+            r[4 * e + 2] = t.x;
+            r[4 * e + 3] = t.y;
+        } else if constexpr (W == 1) {
+            const uint32_t* a = reinterpret_cast<const uint32_t*>(word(e));
+            r[2 * e] = e <= last ? __ldg(a) : 0;
+            r[2 * e + 1] = e <= last ? __ldg(a + 1) : 0;
+        }
+    }
+    return (uint32_t)(reinterpret_cast<uintptr_t>(first) & (N - 1));
+}
+
+template <class IN>
+__device__ __forceinline__ void cut_item(Item<IN>& it, const uint32_t* r, uint32_t off, uint32_t P) {
+    constexpr int W = Item<IN>::W;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t o = off == 8 ? 0 : (off + e * P * W) & (4 * W - 1);
+        if constexpr (W == 2) {
+            const bool high = o & 4;
+            const uint32_t x = high ? r[4 * e + 1] : r[4 * e], y = high ? r[4 * e + 2] : r[4 * e + 1];
+            const uint32_t z = high ? r[4 * e + 3] : r[4 * e + 2];
+            it.w[2 * e] = __funnelshift_r(x, y, (o & 2) * 8);
+            it.w[2 * e + 1] = __funnelshift_r(y, z, (o & 2) * 8);
+        } else if constexpr (W == 1) {
+            it.w[e] = __funnelshift_r(r[2 * e], r[2 * e + 1], o * 8);
         }
     }
 }
@@ -450,7 +519,7 @@ __device__ __forceinline__ void store_item(const Item<IN>& it, char* slot, int c
     char* base = slot + (ch >> 1) * (16 * kAGroup) + (ch & 1) * 128;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int row = vec ? 4 * lane + i : lane + 32 * i;
+        const int row = neighbours<IN>(vec) ? 4 * lane + i : lane + 32 * i;
         uint32_t img[4][SPL];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -491,7 +560,7 @@ __device__ __forceinline__ void copy_item(const Item<T>& it, T* __restrict__ z, 
     for (int e = 0; e < 8; ++e) {
         if (c0 + e >= rows) break;
         T* to = z + (c0 + e) * TP;
-        if (vec) {
+        if (neighbours<T>(vec)) {
             if constexpr (W == 4)
                 *reinterpret_cast<uint4*>(to + 4 * lane) =
                     make_uint4(it.w[4 * e], it.w[4 * e + 1], it.w[4 * e + 2], it.w[4 * e + 3]);
@@ -501,8 +570,6 @@ __device__ __forceinline__ void copy_item(const Item<T>& it, T* __restrict__ z, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (W == 4) to[lane + 32 * i] = __uint_as_float(it.w[4 * e + i]);
-                else
-                    reinterpret_cast<uint16_t*>(to)[lane + 32 * i] = (uint16_t)(it.w[2 * e + i / 2] >> (16 * (i & 1)));
             }
         }
     }
@@ -597,10 +664,20 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
         // The group's place in the sequence of pieces (tile k, chunk j, piece kc), for the loads and for the stores,
         // which run one piece behind; the slot and its phase go with the stores.
         struct Place {
-            int k, j, kc;
+            int k, j, kc, i;
         };
+        // What is in flight: a thread's part of a piece -- or, of a 16-bit field that is not aligned, of one item of it
+        // (the words around its values are twice as many).
+        struct Flight {
+            uint32_t r[32], off[2];
+        };
+        constexpr int W = Item<IN>::W;
+        const bool around = W < 4 && !p.vec;
+        const int units = W == 2 && around ? NI : 1;
         const int chunks = pl.reuse ? 1 : pl.nJ;
         auto advance = [&](Place& q) {
+            if (++q.i < units) return;
+            q.i = 0;
             for (q.kc += kGroups; q.kc >= nA;) {
                 q.kc -= nA;
                 if (++q.j == chunks) {
@@ -609,49 +686,85 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                 }
             }
         };
-        auto load = [&](Item<IN>(&it)[NI], Place& q) {
+        auto load = [&](Flight& f, Place& q) {
             if (q.k >= my) return;
             const bool is_x = !BWD || q.kc < pl.nKx;
             const IN* src = static_cast<const IN*>(is_x ? p.x : p.gy);
             const int k0 = (is_x ? q.kc : q.kc - pl.nKx) * KC;
+            const int rows = is_x ? pl.C : pl.O;
+            const uint32_t n0 = tile_at(q.k) * TP;
+            if constexpr (W == 2) {
+                if (around) {
+                    f.off[0] = load_around<IN>(f.r, src, rows, k0 + (w + 4 * q.i) * 8, n0, lane, p);
+                    advance(q);
+                    return;
+                }
+            }
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-                load_item<IN>(it[i], src, is_x ? pl.C : pl.O, k0 + (w + 4 * i) * 8, tile_at(q.k) * TP, lane, p);
+            for (int i = 0; i < NI; ++i) {
+                if (W == 1 && around) f.off[i] = load_around<IN>(f.r + 16 * i, src, rows, k0 + (w + 4 * i) * 8, n0, lane, p);
+                else load_item<IN>(f.r + (32 / NI) * i, src, rows, k0 + (w + 4 * i) * 8, n0, lane, p);
+            }
             advance(q);
         };
         int slot = group % pl.na;
         uint32_t phase = 1 ^ ((group / pl.na) & 1);       // of the slot's last release: none is needed the first time
-        auto put = [&](const Item<IN>(&it)[NI], Place& q) -> bool {
+        auto put = [&](const Flight& f, Place& q) -> bool {
             if (q.k >= my) return false;
             const bool is_x = !BWD || q.kc < pl.nKx;
             const int pw = is_x ? piece_k(pl.Kx, KC, q.kc) : piece_k(pl.Ky, KC, q.kc - pl.nKx);
-            if (!wait(&bar.empty_a[slot], phase)) return false;  // (a new barrier's phase before the first is complete)
+            if (q.i == 0 && !wait(&bar.empty_a[slot], phase)) return false;  // (true of a new barrier's phase 1)
             char* s = sm + pl.o_a + slot * pl.a_slot;
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
-                if ((w + 4 * i) * 8 < pw) store_item<T, IN>(it[i], s, w + 4 * i, pw / 16, lane, p.vec);
-            if constexpr (BWD) {  // x and e go to the scratch too, once a tile
-                if (p.z && p.z_rows > 3 * pl.H && q.j == 0) {
-                    const int c0 = (is_x ? q.kc : q.kc - pl.nKx) * KC, rows = is_x ? pl.C : pl.O;
-                    T* z = static_cast<T*>(p.z) +
-                           ((int64_t)(tile_at(q.k) - p.tile0) * p.z_rows + 3 * pl.H + (is_x ? 0 : pl.C)) * TP;
-#pragma unroll
-                    for (int i = 0; i < NI; ++i) copy_item<T>(it[i], z, c0 + (w + 4 * i) * 8, rows, lane, p.vec);
+            // x and e go to the scratch too, once a tile
+            const bool keep = BWD && p.z && p.z_rows > 3 * pl.H && q.j == 0;
+            const int c0 = (is_x ? q.kc : q.kc - pl.nKx) * KC;
+            auto one = [&](const Item<IN>& it, int i) {
+                const int ch = w + 4 * i;
+                if (ch * 8 < pw) store_item<T, IN>(it, s, ch, pw / 16, lane, p.vec);
+                if constexpr (BWD) {
+                    if (keep)
+                        copy_item<T>(it,
+                                     static_cast<T*>(p.z) + ((int64_t)(tile_at(q.k) - p.tile0) * p.z_rows + 3 * pl.H +
+                                                             (is_x ? 0 : pl.C)) * TP,
+                                     c0 + ch * 8, is_x ? pl.C : pl.O, lane, p.vec);
+                }
+            };
+            Item<IN> it;
+            bool single = false;
+            if constexpr (W == 2) {
+                if (around) {
+                    single = true;
+                    cut_item<IN>(it, f.r, f.off[0], p.P);
+                    one(it, q.i);
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&bar.full_a[slot]);
-            for (slot += kGroups; slot >= pl.na;) {
-                slot -= pl.na;
-                phase ^= 1;
+            if (!single) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    if (W == 1 && around) {
+                        cut_item<IN>(it, f.r + 16 * i, f.off[i], p.P);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8 * W; ++e) it.w[e] = f.r[(32 / NI) * i + e];
+                    }
+                    one(it, i);
+                }
+            }
+            if (q.i == units - 1) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bar.full_a[slot]);
+                for (slot += kGroups; slot >= pl.na;) {
+                    slot -= pl.na;
+                    phase ^= 1;
+                }
             }
             advance(q);
             return true;
         };
         // the group's next piece is in flight while this one waits for its slot and is written
-        Item<IN> c[NI], d[NI];
-        Place in{0, 0, group - kGroups}, at;
+        Flight c, d;
+        Place in{0, 0, group - kGroups, units - 1}, at;
         advance(in);
         at = in;
         load(c, in);
