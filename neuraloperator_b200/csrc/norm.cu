@@ -30,34 +30,59 @@ namespace rms {
 
 constexpr int kMaxWarps = 16;
 
-template <int BYTES> struct RawOf;
-template <> struct RawOf<1> { using type = uint8_t; };
-template <> struct RawOf<2> { using type = uint16_t; };
-template <> struct RawOf<4> { using type = uint32_t; };
-template <> struct RawOf<8> { using type = uint2; };
-template <> struct RawOf<16> { using type = uint4; };
-
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// V values of type T as they move between memory and registers
+// V values of type T as they move between memory and registers, in 32-bit words: 16-bit values are cut out of them by
+// shifts (through a union with an array they went to local memory, and a bf16 call took as long as an fp32 one)
 template <class T, int V>
 struct Vec {
-    using Raw = typename RawOf<V * sizeof(T)>::type;
-    union U {
-        Raw raw;
-        T e[V];
-        __device__ U() : raw() {}
-    } u;
-    __device__ __forceinline__ void load(const T* p) { u.raw = *reinterpret_cast<const Raw*>(p); }
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = u.raw; }
-    __device__ __forceinline__ float get(int i) const { return to_f(u.e[i]); }
-    __device__ __forceinline__ void set(int i, float v) { u.e[i] = from_f<T>(v); }
+    static constexpr int BYTES = V * (int)sizeof(T), WORDS = BYTES < 4 ? 1 : BYTES / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (BYTES == 2) {
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        } else if constexpr (BYTES == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else if constexpr (BYTES == 8) {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            w[0] = q.x;
+            w[1] = q.y;
+        } else {
+            const uint4 q = *reinterpret_cast<const uint4*>(p);
+            w[0] = q.x;
+            w[1] = q.y;
+            w[2] = q.z;
+            w[3] = q.w;
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (BYTES == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+        else if constexpr (BYTES == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+        else if constexpr (BYTES == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+            return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+        else return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
+    }
+    __device__ __forceinline__ void put(const float (&v)[V]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = __float_as_uint(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) {
+                const float hi = 2 * i + 1 < V ? v[(2 * i + 1) % V] : 0.f;
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], hi);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    const __half2 h = __floats2half2_rn(v[2 * i], hi);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+        }
+    }
 };
 
 // the least power of two s with most <= 448 s, 448 = 0.875 2^9 (1 for a point of zeros, and for one whose
@@ -74,6 +99,14 @@ __device__ __forceinline__ uint8_t to_e4m3(float v) {
     // NaN and infinity become NaN; a value that rounds past 448 by the last bit of the scaling saturates
     return fabsf(v) < INFINITY ? __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3) : (uint8_t)0x7f;
 }
+
+// Threads a CTA has at most, and the CTAs an SM is to hold at least: registers for the NC (with the residual twice as
+// many) loads of up to four words that a thread has in flight, and as many warps as that leaves.
+constexpr int threads_of(int nc) { return nc == 8 ? 256 : 512; }
+constexpr int fwd_ctas(int nc, int words, bool res) {
+    return nc == 8 ? (words == 4 ? (res ? 3 : 4) : words == 2 ? 4 : 6) : nc == 16 ? (words == 1 ? 2 : 1) : 2;
+}
+constexpr int bwd_ctas(int nc, int words) { return nc == 8 ? (words == 1 ? 4 : 3) : nc == 16 ? 1 : 2; }
 
 struct Args {
     const void *x, *res, *gy, *gr;
@@ -115,7 +148,7 @@ __device__ __forceinline__ void meet(float (&s)[V], float* red, int warp, int la
 // RES: 0 no residual, 1 with it.  Q8: the output in 8 bits.  NC: channels a warp holds in registers, 0: none are
 // held and the second pass reads the tile again.
 template <class T, int V, int NC, bool RES, bool Q8>
-__global__ void __launch_bounds__(512) k_fwd(const Args a) {
+__global__ void __launch_bounds__(threads_of(NC), fwd_ctas(NC, Vec<T, V>::WORDS, RES)) k_fwd(const Args a) {
     extern __shared__ float red[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W;
     const int slots = (int)(blockDim.x >> 5) / W;
@@ -134,8 +167,10 @@ __global__ void __launch_bounds__(512) k_fwd(const Args a) {
 
     auto sum_up = [&](Vec<T, V>& v, const Vec<T, V>& u, int c) {
         if (RES) {
+            float t[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v.set(j, v.get(j) + u.get(j));
+            for (int j = 0; j < V; ++j) t[j] = v.get(j) + u.get(j);
+            v.put(t);
             v.store(r + c * a.P);
         }
         const float w = Q8 && a.w ? __ldg(a.w + c) : 1.f;
@@ -150,19 +185,23 @@ __global__ void __launch_bounds__(512) k_fwd(const Args a) {
         }
     };
     if constexpr (NC > 0) {
-        Vec<T, V> u[N];
+        // eight channels at a time: the residual's registers are free again for the next eight
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = cw + i * W;
-            if (valid && c < a.C) {
-                f[i].load(x + c * a.P);
-                if (RES) u[i].load(res + c * a.P);
+        for (int i0 = 0; i0 < N; i0 += 8) {
+            Vec<T, V> u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = cw + (i0 + i) * W;
+                if (valid && c < a.C) {
+                    f[i0 + i].load(x + c * a.P);
+                    if (RES) u[i].load(res + c * a.P);
+                }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = cw + i * W;
-            if (valid && c < a.C) sum_up(f[i], u[i], c);
+            for (int i = 0; i < 8; ++i) {
+                const int c = cw + (i0 + i) * W;
+                if (valid && c < a.C) sum_up(f[i0 + i], u[i], c);
+            }
         }
     } else if (valid) {
 #pragma unroll 4
@@ -193,14 +232,20 @@ __global__ void __launch_bounds__(512) k_fwd(const Args a) {
     auto finish = [&](const Vec<T, V>& v, int c) {
         const float w = a.w ? __ldg(a.w + c) : 1.f;
         if constexpr (Q8) {
-            Vec<uint8_t, V> o;
+            uint32_t o[(V + 3) / 4] = {};
 #pragma unroll
-            for (int j = 0; j < V; ++j) o.u.e[j] = to_e4m3(v.get(j) * inv[j] * w * qs[j]);
-            o.store(a.q + base + c * a.P);
+            for (int j = 0; j < V; ++j) o[j / 4] |= (uint32_t)to_e4m3(v.get(j) * inv[j] * w * qs[j]) << (8 * (j % 4));
+            uint8_t* to = a.q + base + c * a.P;
+            if constexpr (V == 1) *to = (uint8_t)o[0];
+            else if constexpr (V == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)o[0];
+            else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(to) = o[0];
+            else *reinterpret_cast<uint2*>(to) = make_uint2(o[0], o[1]);
         } else {
-            Vec<T, V> o;
+            float t[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) o.set(j, v.get(j) * inv[j] * w);
+            for (int j = 0; j < V; ++j) t[j] = v.get(j) * inv[j] * w;
+            Vec<T, V> o;
+            o.put(t);
             o.store(static_cast<T*>(a.y) + base + c * a.P);
         }
     };
@@ -225,7 +270,7 @@ __global__ void __launch_bounds__(512) k_fwd(const Args a) {
 // partial sums [slot of the grid][C] are few and are added in a fixed order (k_reduce).  NC = 0: the channels'
 // sums are kept in shared memory (one warp owns a channel) and the lanes meet in every tile.
 template <class T, int V, int NC, bool GR>
-__global__ void __launch_bounds__(512) k_bwd(const Args a) {
+__global__ void __launch_bounds__(threads_of(NC), bwd_ctas(NC, Vec<T, V>::WORDS)) k_bwd(const Args a) {
     extern __shared__ float red[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, warps = blockDim.x >> 5;
     const int slots = warps / W, slot = warp / W, cw = warp % W;
@@ -235,6 +280,7 @@ __global__ void __launch_bounds__(512) k_bwd(const Args a) {
         __syncthreads();
     }
     constexpr int N = NC ? NC : 1;
+    constexpr bool kHoldR = NC == 8;  // dL/dr of the residual's path comes with the first loads (registers for 8 channels)
     float gw[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) gw[i] = 0.f;
@@ -247,7 +293,7 @@ __global__ void __launch_bounds__(512) k_bwd(const Args a) {
         const int64_t g = (t0 + slot) * 32 + lane;
         const bool valid = g < a.groups;
         const int64_t base = valid ? base_of<V>(a, g) : 0;
-        Vec<T, V> f[N], d[N];
+        Vec<T, V> f[N], d[N], r[N];
         float s1[V], s2[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
@@ -266,6 +312,7 @@ __global__ void __launch_bounds__(512) k_bwd(const Args a) {
                 if (valid && c < a.C) {
                     f[i].load(px + base + c * a.P);
                     d[i].load(pg + base + c * a.P);
+                    if (GR && kHoldR) r[i].load(pr + base + c * a.P);
                 }
             }
 #pragma unroll
@@ -297,17 +344,19 @@ __global__ void __launch_bounds__(512) k_bwd(const Args a) {
             inv[j] = 1.f / sqrtf(s1[j] / (float)a.C + a.eps);
             back[j] = inv[j] * inv[j] * (t / (float)a.C);  // inv m
         }
-        auto finish = [&](const Vec<T, V>& v, const Vec<T, V>& e, int c) -> float {
+        auto finish = [&](const Vec<T, V>& v, const Vec<T, V>& e, Vec<T, V> u, int c) -> float {
             const float w = a.w ? __ldg(a.w + c) : 1.f;
-            Vec<T, V> u, o;
-            if (GR) u.load(pr + base + c * a.P);
+            float q[V];
+            if (GR && !kHoldR) u.load(pr + base + c * a.P);
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 sum = fmaf(e.get(j), v.get(j) * inv[j], sum);
                 const float t = inv[j] * (e.get(j) * w - v.get(j) * back[j]);
-                o.set(j, GR ? t + u.get(j) : t);
+                q[j] = GR ? t + u.get(j) : t;
             }
+            Vec<T, V> o;
+            o.put(q);
             if (po) o.store(po + base + c * a.P);
             return sum;
         };
@@ -315,7 +364,7 @@ __global__ void __launch_bounds__(512) k_bwd(const Args a) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int c = cw + i * W;
-                if (valid && c < a.C) gw[i] += finish(f[i], d[i], c);
+                if (valid && c < a.C) gw[i] += finish(f[i], d[i], r[i], c);
             }
         } else {
             for (int c = cw; c < a.C; c += W) {
@@ -324,7 +373,7 @@ __global__ void __launch_bounds__(512) k_bwd(const Args a) {
                     Vec<T, V> v, e;
                     v.load(px + base + c * a.P);
                     e.load(pg + base + c * a.P);
-                    sum = finish(v, e, c);
+                    sum = finish(v, e, Vec<T, V>(), c);
                 }
                 if (a.partial) {
 #pragma unroll
@@ -371,8 +420,9 @@ constexpr int kMaxSms = 160;         // CTAs are planned for at most so many mul
 struct Cut {
     int V, W, NC, warps;
     int64_t groups, tiles;
-    // the backward's persistent CTAs: a few an SM, 32 warps' worth of registers
-    int max_grid(int sms) const { return (sms < kMaxSms ? sms : kMaxSms) * (warps > 8 ? 2 : 4); }
+    // the backward's CTAs: with 8 channels a warp a few times what an SM holds, so that the last ones to end are a small
+    // part (12 an SM against 4: 557 -> 444 us at 64 channels, 2^21 points); with 16 the sums at a CTA's end cost more
+    int max_grid(int sms) const { return (sms < kMaxSms ? sms : kMaxSms) * (NC == 8 ? 12 : warps > 8 ? 2 : 4); }
 };
 
 // V: the widest load of up to 16 bytes that the points per sample and every pointer allow; one point a thread
