@@ -11,7 +11,7 @@ from .fno import FNO, TFNO  # noqa: F401
 from .fno_block import FNOBlocks  # noqa: F401
 from .fno_staged import FNOStaged  # noqa: F401
 from .gated import gated_mlp  # noqa: F401
-from .layers import ChannelMLP, GridEmbeddingND, SoftGating, skip_connection  # noqa: F401
+from .layers import ChannelMLP, GatedChannelMLP, GridEmbeddingND, SoftGating, skip_connection  # noqa: F401
 from .norm import RMSNorm, rms_norm, rms_norm_quantized  # noqa: F401
 from .spectral_convolution import BaseSpectralConv, SpectralConv  # noqa: F401
 from .utils import count_model_params  # noqa: F401

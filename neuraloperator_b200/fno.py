@@ -6,7 +6,9 @@ the default layer shapes the grid embedding + lifting is one per-pixel tensor-co
 (``pointwise.chain``), every block is its spectral convolution plus one such kernel, and the
 projection is fused into the last block's kernel.
 Options the reference offers outside the FNO default path raise NotImplementedError here:
-``domain_padding``, ``norm``, ``complex_data`` and ``fno_block_precision`` other than "full".
+``domain_padding``, the reference's ``norm`` layers, ``complex_data`` and ``fno_block_precision`` other than "full".
+``norm="rms_norm"`` and ``channel_mlp_type="gated"`` (FNOBlocks) run the blocks layer by layer on this library's
+kernels, with the lifting and the projection still one kernel each.
 """
 
 from __future__ import annotations
@@ -39,7 +41,7 @@ class FNO(nn.Module):
                  rank: float = 1.0, fixed_rank_modes: bool = False, implementation: str = "factorized",
                  decomposition_kwargs: dict = None, separable: bool = False, preactivation: bool = False,
                  conv_module: nn.Module = SpectralConv, enforce_hermitian_symmetry: bool = True,
-                 contraction_precision: str = "fp32", engine: str = "auto"):
+                 contraction_precision: str = "fp32", engine: str = "auto", channel_mlp_type: str = "mlp"):
         super().__init__()
         if decomposition_kwargs is None:
             decomposition_kwargs = {}
@@ -94,7 +96,7 @@ class FNO(nn.Module):
             fixed_rank_modes=fixed_rank_modes, implementation=implementation, separable=separable,
             factorization=factorization, decomposition_kwargs=decomposition_kwargs, conv_module=conv_module,
             n_layers=n_layers, enforce_hermitian_symmetry=enforce_hermitian_symmetry,
-            contraction_precision=contraction_precision, engine=engine)
+            contraction_precision=contraction_precision, engine=engine, channel_mlp_type=channel_mlp_type)
         lifting_in = in_channels + (self.n_dim if self.positional_embedding is not None else 0)
         self.lifting = ChannelMLP(in_channels=lifting_in, out_channels=hidden_channels,
                                   hidden_channels=self.lifting_channels, n_layers=2, n_dim=self.n_dim,
@@ -174,13 +176,39 @@ class FNO(nn.Module):
             output_shape = [None] * self.n_layers
         elif isinstance(output_shape, tuple):
             output_shape = [None] * (self.n_layers - 1) + [output_shape]
-        if self.positional_embedding is not None:
-            x = self.positional_embedding(x)
-        x = self.lifting(x)
+        # blocks with norms or gates are no chains, but the layers around them are
+        around = self.fno_blocks.norm is not None or self.fno_blocks.channel_mlp_type == "gated"
+        lifted = self._chain_lifting(x) if around else None
+        if lifted is None:
+            if self.positional_embedding is not None:
+                x = self.positional_embedding(x)
+            lifted = self.lifting(x)
+        x = lifted
         for i in range(self.n_layers):
             x = self.fno_blocks(x, i, output_shape=output_shape[i])
-        x = self.projection(x)
-        return x
+        y = self._chain_mlp(self.projection, x) if around else None
+        return self.projection(x) if y is None else y
+
+    def _chain_mlp(self, mlp, x, grid=None):
+        """A ChannelMLP (with `grid`, of x and the grid's coordinates) as one chain kernel; None when it does not fit."""
+        if not (self._mlp_ok(mlp) and x.is_cuda and x.dtype == torch.float32):
+            return None
+        f1, f2 = mlp.fcs
+        args = (x.shape[0], tuple(x.shape[2:]), x.shape[1], f1.out_channels, f2.out_channels)
+        if not pointwise.supported(*args, grid=grid) or (
+                grad_needed(x, mlp) and not pointwise.backward_supported(*args, grid=grid)):
+            return None
+        return pointwise.chain(x, f1.weight, f1.bias, f2.weight, f2.bias, grid=grid)
+
+    def _chain_lifting(self, x):
+        pe = self.positional_embedding
+        if (pe is not None and not isinstance(pe, GridEmbeddingND)) or x.ndim != 2 + self.n_dim:
+            return None
+        if x.shape[1] != self.in_channels or self.lifting.in_channels != self.in_channels + (
+                self.n_dim if pe is not None else 0):
+            return None
+        grid = pointwise.grid_params(pe.grid_boundaries, tuple(x.shape[2:])) if pe is not None else None
+        return self._chain_mlp(self.lifting, x, grid)
 
     @torch.no_grad()
     def forward_host(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, chunk: Optional[int] = None,

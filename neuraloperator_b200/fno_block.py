@@ -8,7 +8,10 @@ soft-gating (or no) channel-MLP skip -- it runs as two launch sequences: the spe
 the linear skip W_skip x to the spectral output, applies GELU, the ChannelMLP, the soft-gating skip of x
 and the closing GELU (:339-381).  x is read twice from HBM and the block output written once.  Every
 other configuration composes the same operations as the reference around the CUDA spectral block.
-Normalisation layers other than None are not provided (norm=None is the FNO default).
+``norm="rms_norm"`` puts this package's RMSNorm where the reference has its norms (after the spectral convolution and,
+with the addition of the channel-MLP skip in the same kernel, after the channel MLP; preactivation: before the
+convolution and before the channel MLP); the reference's own normalisation layers are not provided (norm=None is the
+FNO default).  ``channel_mlp_type="gated"`` makes the channel MLPs GatedChannelMLPs.
 """
 
 from __future__ import annotations
@@ -20,7 +23,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import pointwise
-from .layers import ChannelMLP, SoftGating, skip_connection
+from .layers import ChannelMLP, GatedChannelMLP, SoftGating, skip_connection
+from .norm import RMSNorm
 from .spectral_convolution import SpectralConv
 from .utils import grad_needed, validate_scaling_factor
 
@@ -34,7 +38,7 @@ class FNOBlocks(nn.Module):
                  ada_in_features=None, preactivation=False, fno_skip="linear", channel_mlp_skip="soft-gating",
                  complex_data=False, separable=False, factorization=None, rank=1.0, conv_module=SpectralConv,
                  fixed_rank_modes=False, implementation="factorized", decomposition_kwargs=dict(),
-                 enforce_hermitian_symmetry=True, contraction_precision="fp32", engine="auto"):
+                 enforce_hermitian_symmetry=True, contraction_precision="fp32", engine="auto", channel_mlp_type="mlp"):
         super().__init__()
         if isinstance(n_modes, int):
             n_modes = [n_modes]
@@ -65,10 +69,18 @@ class FNOBlocks(nn.Module):
         if complex_data:
             raise NotImplementedError("FNOBlocks with complex_data is not provided; SpectralConv supports "
                                       "complex data on its own")
-        if norm is not None:
-            raise NotImplementedError(f"norm={norm!r} is not provided (the FNO default is norm=None)")
-        self.norm = None
+        if norm not in (None, "rms_norm"):
+            raise NotImplementedError(f"norm={norm!r} is not provided (None, the FNO default, or 'rms_norm')")
         self.n_norms = 2
+        self.norm = (nn.ModuleList([RMSNorm(out_channels) for _ in range(self.n_norms * n_layers)])
+                     if norm == "rms_norm" else None)
+        if preactivation and norm == "rms_norm" and in_channels != out_channels:
+            raise ValueError("preactivation norms the block's input and output: in_channels must equal out_channels")
+        if channel_mlp_type not in ("mlp", "gated"):
+            raise ValueError(f"channel_mlp_type must be 'mlp' or 'gated', got {channel_mlp_type!r}")
+        if channel_mlp_type == "gated" and channel_mlp_dropout:
+            raise ValueError("channel_mlp_type='gated' has no dropout")
+        self.channel_mlp_type = channel_mlp_type
         self.non_linearity = non_linearity
         ours = isinstance(conv_module, type) and issubclass(conv_module, SpectralConv)
         extra = {"enforce_hermitian_symmetry": enforce_hermitian_symmetry} if ours else {}
@@ -87,8 +99,11 @@ class FNOBlocks(nn.Module):
                                                          n_dim=self.n_dim) for _ in range(n_layers)])
                           if fno_skip is not None else None)
         if use_channel_mlp:
+            hidden = round(self.out_channels * channel_mlp_expansion)
             self.channel_mlp = nn.ModuleList([
-                ChannelMLP(in_channels=self.out_channels, hidden_channels=round(self.out_channels * channel_mlp_expansion),
+                GatedChannelMLP(in_channels=self.out_channels, hidden_channels=hidden, n_dim=self.n_dim)
+                if channel_mlp_type == "gated" else
+                ChannelMLP(in_channels=self.out_channels, hidden_channels=hidden,
                            dropout=channel_mlp_dropout, n_dim=self.n_dim) for _ in range(n_layers)])
             self.channel_mlp_skips = (nn.ModuleList([
                 skip_connection(self.in_channels, self.out_channels, skip_type=channel_mlp_skip, n_dim=self.n_dim)
@@ -103,7 +118,7 @@ class FNOBlocks(nn.Module):
         """The spectral convolution of block `index` runs bare (no resampling) and its linear skip, GELU
         and the rest of the block can be composed around it."""
         conv = self.convs[index]
-        return (isinstance(conv, SpectralConv) and self.fno_skips is not None and self.fno_skip.lower() == "linear"
+        return (isinstance(conv, SpectralConv) and self.norm is None and self.fno_skips is not None and self.fno_skip.lower() == "linear"
                 and self.stabilizer is None and self.non_linearity is F.gelu and output_shape is None
                 and conv.resolution_scaling_factor is None and x.is_cuda)
 
@@ -183,19 +198,29 @@ class FNOBlocks(nn.Module):
             if self.stabilizer == "tanh":
                 x = torch.tanh(x)
             x_fno = self.convs[index](x, output_shape=output_shape)
+            if self.norm is not None:
+                x_fno = self.norm[self.n_norms * index](x_fno)
             x = x_fno + x_skip if self.fno_skips is not None else x_fno
             if not last:
                 x = self.non_linearity(x)
+        skip = None
         if self.use_channel_mlp:
             x = self.channel_mlp[index](x)
             if self.channel_mlp_skips is not None:
-                x = x + x_skip_mlp
+                skip = x_skip_mlp
+        if self.norm is not None:
+            norm = self.norm[self.n_norms * index + 1]
+            x = norm(x) if skip is None else norm(x, residual=skip)[0]
+        elif skip is not None:
+            x = x + skip
         if not last:
             x = self.non_linearity(x)
         return x
 
     def forward_with_preactivation(self, x, index=0, output_shape=None):
         x = self.non_linearity(x)
+        if self.norm is not None:
+            x = self.norm[self.n_norms * index](x)
         if self.fno_skips is not None:
             x_skip = self.convs[index].transform(self.fno_skips[index](x), output_shape=output_shape)
         if self.use_channel_mlp and self.channel_mlp_skips is not None:
@@ -207,6 +232,8 @@ class FNOBlocks(nn.Module):
         if index < self.n_layers - 1:
             x = self.non_linearity(x)
         if self.use_channel_mlp:
+            if self.norm is not None:
+                x = self.norm[self.n_norms * index + 1](x)
             x = self.channel_mlp[index](x)
             if self.channel_mlp_skips is not None:
                 x = x + x_skip_mlp

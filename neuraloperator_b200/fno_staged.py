@@ -42,7 +42,7 @@ class FNOStaged(FNO):
                  fixed_rank_modes: bool = False, implementation: str = "factorized",
                  decomposition_kwargs: dict = None, separable: bool = False, preactivation: bool = False,
                  conv_module: nn.Module = SpectralConv, enforce_hermitian_symmetry: bool = True, no_br: bool = False,
-                 contraction_precision: str = "fp32", engine: str = "auto"):
+                 contraction_precision: str = "fp32", engine: str = "auto", channel_mlp_type: str = "mlp"):
         if n_layers is not None and n_layers != len(n_modes_per_layer):
             raise ValueError(f"Got n_layers={n_layers} but n_modes_per_layer has length {len(n_modes_per_layer)}")
         if no_br:
@@ -69,7 +69,7 @@ class FNOStaged(FNO):
             implementation=implementation, decomposition_kwargs=decomposition_kwargs, separable=separable,
             preactivation=preactivation, conv_module=conv_module,
             enforce_hermitian_symmetry=enforce_hermitian_symmetry, contraction_precision=contraction_precision,
-            engine=engine)
+            engine=engine, channel_mlp_type=channel_mlp_type)
         self.no_br = no_br
         self.n_modes_per_layer = [list(m) for m in modes]
         self.max_n_modes_per_layer = [list(m) for m in max_modes]

@@ -4,7 +4,8 @@ ChannelMLP (neuralop/layers/channel_mlp.py:6-119), skip connections
 (neuralop/layers/skip_connections.py:5-127), GridEmbeddingND (neuralop/layers/embeddings.py:90-164,
 351-383) and resample (neuralop/layers/resample.py:7-80).  These are per-pixel channel GEMMs,
 elementwise ops and interpolation; they run as PyTorch (cuBLAS / cuDNN) ops on the device.
-Parameter names match the reference so its state dicts load.
+Parameter names match the reference so its state dicts load.  GatedChannelMLP, which the reference does not have, is a
+ChannelMLP with a gate; it runs on this library's kernels.
 """
 
 from __future__ import annotations
@@ -15,6 +16,8 @@ from typing import List
 import torch
 import torch.nn.functional as F
 from torch import nn
+
+from .gated import MAX_CHANNELS, MAX_HIDDEN, gated_mlp
 
 
 class ChannelMLP(nn.Module):
@@ -75,6 +78,30 @@ class Flattened1dConv(nn.Module):
         x = x.view(*size[:2], -1)
         x = self.conv(x)
         return x.view(size[0], self.conv.out_channels, *size[2:])
+
+
+class GatedChannelMLP(nn.Module):
+    """Gated feed-forward layer at every point, ``down(act(gate(x)) * up(x))``: a ChannelMLP whose hidden layer is a
+    product of two projections (``gated.gated_mlp``; forward and backward on the tensor cores).  ``gate``, ``up`` and
+    ``down`` are Conv1d layers of kernel size 1, as in ChannelMLP.  At most 256 channels."""
+
+    def __init__(self, in_channels, out_channels=None, hidden_channels=None, n_dim=2, activation="silu", bias=True):
+        super().__init__()
+        self.in_channels = in_channels
+        self.out_channels = in_channels if out_channels is None else out_channels
+        self.hidden_channels = in_channels if hidden_channels is None else hidden_channels
+        self.activation = activation
+        if not (1 <= self.in_channels <= MAX_CHANNELS and 1 <= self.out_channels <= MAX_CHANNELS
+                and 1 <= self.hidden_channels <= MAX_HIDDEN):
+            raise ValueError(f"GatedChannelMLP takes 1..{MAX_CHANNELS} channels and a hidden width of 1..{MAX_HIDDEN}, "
+                             f"got {self.in_channels} -> {self.hidden_channels} -> {self.out_channels}")
+        self.gate = nn.Conv1d(self.in_channels, self.hidden_channels, 1, bias=bias)
+        self.up = nn.Conv1d(self.in_channels, self.hidden_channels, 1, bias=bias)
+        self.down = nn.Conv1d(self.hidden_channels, self.out_channels, 1, bias=bias)
+
+    def forward(self, x, x_scale=None):
+        return gated_mlp(x, self.gate.weight, self.up.weight, self.down.weight, self.gate.bias, self.up.bias,
+                         self.down.bias, activation=self.activation, x_scale=x_scale)
 
 
 def skip_connection(in_features, out_features, n_dim=2, bias=False, skip_type="soft-gating"):

@@ -188,3 +188,20 @@ def test_gated_pointers():
     assert lib.nop_gated_backward(d, ops(), _lib.NopGatedGrads(gy=512, gx=513), 512, 1 << 30, None) == -3
     assert lib.nop_gated_backward(d, ops(), _lib.NopGatedGrads(gy=512, gx=512), 512, 8, None) == -4
     assert lib.nop_gated_backward(gated_desc(dtype=1, x_dtype=3), ops(), g, 512, 1 << 30, None) == -2
+
+
+def test_block_options():
+    kw = dict(n_modes=(4, 4), in_channels=1, out_channels=1, hidden_channels=8)
+    with pytest.raises(NotImplementedError, match="norm"):
+        nb.FNO(**kw, norm="group_norm")
+    with pytest.raises(ValueError, match="channel_mlp_type"):
+        nb.FNO(**kw, channel_mlp_type="glu")
+    with pytest.raises(ValueError, match="dropout"):
+        nb.FNO(**kw, channel_mlp_type="gated", channel_mlp_dropout=0.1)
+    with pytest.raises(ValueError, match="channels"):
+        nb.GatedChannelMLP(300)
+    model = nb.FNO(**kw, n_layers=3, norm="rms_norm", channel_mlp_type="gated")
+    assert len(model.fno_blocks.norm) == 6 and isinstance(model.fno_blocks.channel_mlp[0], nb.GatedChannelMLP)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        model(fake(1, 1, 8, 8))
+    assert nb.FNO(**kw).fno_blocks.norm is None  # the default is as it was
