@@ -35,15 +35,15 @@ def _limit(max_norm: float) -> float:
 
 
 def _check(tensors: Sequence[torch.Tensor]) -> torch.device:
-    dev = tensors[0].device
-    for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError("neuraloperator_b200 runs on CUDA devices only (there is no CPU path)")
-        if t.dtype not in _DTYPES:
-            raise TypeError(f"expected float32, bfloat16, float16 or complex64 tensors, got {t.dtype}")
-        if t.device != dev:
-            raise ValueError("all tensors must be on one device")
-    return dev
+    devices = {t.device for t in tensors}
+    if any(d.type != "cuda" for d in devices):
+        raise RuntimeError("neuraloperator_b200 runs on CUDA devices only (there is no CPU path)")
+    for dtype in {t.dtype for t in tensors}:
+        if dtype not in _DTYPES:
+            raise TypeError(f"expected float32, bfloat16, float16 or complex64 tensors, got {dtype}")
+    if len(devices) > 1:
+        raise ValueError("all tensors must be on one device")
+    return devices.pop()
 
 
 def _run(src: List[torch.Tensor], dst, max_norm: float, kind: int, dev: torch.device) -> torch.Tensor:
@@ -57,8 +57,9 @@ def _run(src: List[torch.Tensor], dst, max_norm: float, kind: int, dev: torch.de
     pointers = ctypes.c_void_p * n
     a = pointers(*[t.data_ptr() for t in src])
     b = a if dst is src else None if dst is None else pointers(*[t.data_ptr() for t in dst])
-    numel = (ctypes.c_int64 * n)(*[2 * t.numel() if t.is_complex() else t.numel() for t in src])
-    dtypes = (ctypes.c_int32 * n)(*[_DTYPES[t.dtype] for t in src])
+    kinds = [t.dtype for t in src]
+    numel = (ctypes.c_int64 * n)(*[2 * t.numel() if k is torch.complex64 else t.numel() for t, k in zip(src, kinds)])
+    dtypes = (ctypes.c_int32 * n)(*[_DTYPES[k] for k in kinds])
     _lib.call(lib.nop_clip_by_norm, dev, n, a, b, numel, dtypes, kind, max_norm, norm.data_ptr(), ws.data_ptr(),
               size.value)
     return norm
@@ -83,7 +84,7 @@ def clip_by_global_norm(tensors: Iterable[torch.Tensor], max_norm: float,
     if not tensors:
         return [], torch.zeros(())
     dev = _check(tensors)
-    src = [t.resolve_conj().contiguous() for t in tensors]
+    src = [t if t.is_contiguous() and not t.is_conj() else t.resolve_conj().contiguous() for t in tensors]
     dst = [torch.empty_like(t) for t in src]
     return dst, _run(src, dst, limit, kind, dev)
 

@@ -83,7 +83,7 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if t is None else t.detach().contiguous()
+    return t if t is None or (t.is_contiguous() and not t.requires_grad) else t.detach().contiguous()
 
 
 def _workspace(lib, desc, backward: int, device) -> torch.Tensor:

@@ -50,8 +50,14 @@ def _desc(x: torch.Tensor, eps: float) -> _lib.NopNormDesc:
     return _lib.NopNormDesc(_lib.ABI_VERSION, _DTYPES[x.dtype], batch, points, channels, eps)
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() and not t.requires_grad else t.detach().contiguous()
+
+
 def _fp32(weight: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if weight is None else weight.detach().to(torch.float32).contiguous()
+    if weight is None or (weight.dtype is torch.float32 and weight.is_contiguous()):
+        return weight
+    return weight.detach().to(torch.float32).contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -60,8 +66,8 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _forward(x, weight, residual, eps):
     """(y, r): r is x itself without a residual."""
-    x = x.detach().contiguous()
-    residual = None if residual is None else residual.detach().contiguous()
+    x = _dense(x)
+    residual = None if residual is None else _dense(residual)
     y = torch.empty_like(x)
     r = x if residual is None else torch.empty_like(x)
     w = _fp32(weight)
@@ -124,8 +130,8 @@ def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_quantized has no backward; call it under torch.no_grad()")
-    x = x.detach().contiguous()
-    residual = None if residual is None else residual.detach().contiguous()
+    x = _dense(x)
+    residual = None if residual is None else _dense(residual)
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty((x.shape[0], 1, *x.shape[2:]), device=x.device, dtype=torch.float32)
     r = None if residual is None else torch.empty_like(x)
