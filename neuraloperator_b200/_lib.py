@@ -303,7 +303,7 @@ def check(code: int):
 def call(fn, device, *args):
     """fn(*args, stream) on ``device`` (a torch CUDA device) and its current stream, its status checked."""
     import torch
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(device.index)  # current_stream(device).cuda_stream without its object
     if torch.cuda.current_device() == device.index:
         code = fn(*args, stream)
     else:

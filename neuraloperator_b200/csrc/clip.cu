@@ -19,6 +19,19 @@
 #include <exception>
 
 namespace nop {
+
+int32_t current_device(int* dev, int* sms) {
+    static std::atomic<int> known[64];
+    NOP_CUDA_TRY(cudaGetDevice(dev));
+    int n = *dev < 64 ? known[*dev].load(std::memory_order_relaxed) : 0;
+    if (!n) {
+        NOP_CUDA_TRY(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev));
+        if (*dev < 64) known[*dev].store(n, std::memory_order_relaxed);
+    }
+    *sms = n;
+    return NOP_OK;
+}
+
 namespace clip {
 
 constexpr int kItems = 256;         // tensors a launch (a 32-byte entry each in the kernel parameters)
@@ -263,8 +276,8 @@ int32_t nop_clip_by_norm(int32_t n, const void* const* src, void* const* dst, co
     if (tables.size() * clip::kMaxGrid * sizeof(double) > workspace_bytes)
         return fail(NOP_E_WORKSPACE, "workspace too small");
     int dev = 0, sms = 148;
-    NOP_CUDA_TRY(cudaGetDevice(&dev));
-    NOP_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    const int32_t dc = current_device(&dev, &sms);
+    if (dc != NOP_OK) return dc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     double* partial = static_cast<double*>(workspace);
     return norm_type == NOP_NORM_INF ? clip::run<true>(tables, dst != nullptr, max_norm, norm, partial, sms, s)

@@ -1626,22 +1626,22 @@ int32_t by_type(int dtype, F&& f) {
 }
 
 struct Device {
-    int sms = 148;
+    int dev = 0, sms = 148;
     int* status = nullptr;
 };
 int32_t device(Device* d) {
-    int dev = 0;
-    NOP_CUDA_TRY(cudaGetDevice(&dev));
-    NOP_CUDA_TRY(cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, dev));
-    d->status = status_word(dev);
+    const int32_t rc = current_device(&d->dev, &d->sms);
+    if (rc != NOP_OK) return rc;
+    d->status = status_word(d->dev);
     if (!d->status) return fail(NOP_E_CUDA, "status word of the tensor-core kernels is not available");
     return NOP_OK;
 }
 
-template <class K, class... A>
-int32_t launch(K kernel, unsigned grid, int threads, int smem, cudaStream_t s, A... args) {
-    NOP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<grid, threads, smem, s>>>(args...);
+template <auto KERNEL, class... A>
+int32_t launch(const Device& d, unsigned grid, int threads, int smem, cudaStream_t s, A... args) {
+    const int32_t rc = allow_smem<KERNEL>(d.dev, kSmem);
+    if (rc != NOP_OK) return rc;
+    KERNEL<<<grid, threads, smem, s>>>(args...);
     NOP_CUDA_TRY(cudaGetLastError());
     return NOP_OK;
 }
@@ -1714,8 +1714,8 @@ int32_t forward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, co
         q.out = o.y;
         q.vec = d.points % 4 == 0 && aligned({o.x}, 4 * sizeof(IN));
         rc = d.activation == NOP_ACT_GELU
-                 ? launch(k_block<T, IN, false, true>, grid, Roles<false>::THREADS, p.smem, s, q, dev.status)
-                 : launch(k_block<T, IN, false, false>, grid, Roles<false>::THREADS, p.smem, s, q, dev.status);
+                 ? launch<k_block<T, IN, false, true>>(dev, grid, Roles<false>::THREADS, p.smem, s, q, dev.status)
+                 : launch<k_block<T, IN, false, false>>(dev, grid, Roles<false>::THREADS, p.smem, s, q, dev.status);
         if (rc != NOP_OK || p.col0 + p.cols >= p.O) return rc;
         if (!make_plan<T>(d, false, p.col0 + p.cols, &p)) return fail(NOP_E_UNSUPPORTED, kTooLarge);
     }
@@ -1769,14 +1769,14 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
         q.tile0 = (int)t;
         q.tiles = (int)std::min<int64_t>(slab, z.tiles - t);
         const unsigned grid = (unsigned)std::min<int64_t>(q.tiles, dev.sms);
-        rc = d.activation == NOP_ACT_GELU ? launch(k_block<T, T, true, true>, grid, Roles<true>::THREADS, p.smem, s, q, dev.status)
-                                          : launch(k_block<T, T, true, false>, grid, Roles<true>::THREADS, p.smem, s, q, dev.status);
+        rc = d.activation == NOP_ACT_GELU ? launch<k_block<T, T, true, true>>(dev, grid, Roles<true>::THREADS, p.smem, s, q, dev.status)
+                                          : launch<k_block<T, T, true, false>>(dev, grid, Roles<true>::THREADS, p.smem, s, q, dev.status);
         if (rc != NOP_OK) return rc;
         if (!weights) continue;
         w.pieces = q.tiles * (TP / WForm<T>::KC);
         w.tile0 = (int)t;
         w.accumulate = t > 0;
-        rc = launch(k_wgrad<T>, (unsigned)(z.splits * z.wtiles), WForm<T>::THREADS, wsmem, s, mg, mh, mx, me, w, dev.status);
+        rc = launch<k_wgrad<T>>(dev, (unsigned)(z.splits * z.wtiles), WForm<T>::THREADS, wsmem, s, mg, mh, mx, me, w, dev.status);
         if (rc != NOP_OK) return rc;
     }
     // dL/dx of the channels past the first launch's: the products again, without the scratch
@@ -1788,8 +1788,8 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
         r.out = q.out;
         r.vec = q.vec;
         const unsigned grid = (unsigned)std::min<int64_t>(z.tiles, dev.sms);
-        rc = d.activation == NOP_ACT_GELU ? launch(k_block<T, T, true, true>, grid, Roles<true>::THREADS, p.smem, s, r, dev.status)
-                                          : launch(k_block<T, T, true, false>, grid, Roles<true>::THREADS, p.smem, s, r, dev.status);
+        rc = d.activation == NOP_ACT_GELU ? launch<k_block<T, T, true, true>>(dev, grid, Roles<true>::THREADS, p.smem, s, r, dev.status)
+                                          : launch<k_block<T, T, true, false>>(dev, grid, Roles<true>::THREADS, p.smem, s, r, dev.status);
         if (rc != NOP_OK) return rc;
     }
     if (!weights) return NOP_OK;

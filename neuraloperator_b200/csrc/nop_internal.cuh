@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -133,6 +134,20 @@ int32_t spectrum_layout(const Plan& p, int64_t* q_stride, int64_t* b_stride, int
 size_t weight_grad_workspace(const Plan& p);
 int32_t weight_grad(const Plan& p, const void* x_spec, const Plan& adjoint, const void* g_spec, void* grad_w,
                     float* grad_bias, void* workspace, size_t workspace_bytes, cudaStream_t s);
+
+// The current device and its multiprocessors (asked of the runtime once a device).
+int32_t current_device(int* dev, int* sms);
+
+// Lets the kernel take `bytes` of dynamic shared memory on device `dev`; asked of the runtime once a kernel and device.
+template <auto KERNEL>
+int32_t allow_smem(int dev, int bytes) {
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return NOP_OK;
+    NOP_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+    return NOP_OK;
+}
 
 // ------------------------------------------------------------------------------------------
 // small device helpers

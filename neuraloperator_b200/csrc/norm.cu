@@ -485,16 +485,16 @@ int32_t launch_fwd(const Args& a, const Cut& c, bool residual, bool q8, cudaStre
 }
 
 template <class T, int V, int NC>
-int32_t launch_bwd(const Args& a, const Cut& c, unsigned grid, cudaStream_t s) {
+int32_t launch_bwd(const Args& a, const Cut& c, unsigned grid, int dev, cudaStream_t s) {
     const int smem = (4 * c.warps * 32 * V + (NC ? 0 : a.C)) * 4;
     const int threads = c.warps * 32;
-    if (a.gr) {
-        NOP_CUDA_TRY(cudaFuncSetAttribute(k_bwd<T, V, NC, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        k_bwd<T, V, NC, true><<<grid, threads, smem, s>>>(a);
-    } else {
-        NOP_CUDA_TRY(cudaFuncSetAttribute(k_bwd<T, V, NC, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        k_bwd<T, V, NC, false><<<grid, threads, smem, s>>>(a);
+    if (smem > 48 * 1024) {  // (with the sums of many channels)
+        constexpr int most = (4 * kMaxWarps * 32 * V + kMaxChannels) * 4;
+        const int32_t rc = a.gr ? allow_smem<k_bwd<T, V, NC, true>>(dev, most) : allow_smem<k_bwd<T, V, NC, false>>(dev, most);
+        if (rc != NOP_OK) return rc;
     }
+    if (a.gr) k_bwd<T, V, NC, true><<<grid, threads, smem, s>>>(a);
+    else k_bwd<T, V, NC, false><<<grid, threads, smem, s>>>(a);
     NOP_CUDA_TRY(cudaGetLastError());
     return NOP_OK;
 }
@@ -529,13 +529,6 @@ int32_t dispatch(int dtype, const Cut& c, F&& f) {
     return by_v(__half{});
 }
 
-int32_t device_sms(int* sms) {
-    int dev = 0;
-    NOP_CUDA_TRY(cudaGetDevice(&dev));
-    NOP_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
-    return NOP_OK;
-}
-
 // every pointer on a 16-byte boundary (wide loads), or at least on its type's
 bool on_16(std::initializer_list<const void*> ps) {
     uintptr_t all = 0;
@@ -564,8 +557,8 @@ int32_t nop_rms_norm_forward(const nop_norm_desc* d, const void* x, const void* 
     if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y | (uintptr_t)r) % size || (uintptr_t)scale % 4 ||
         (uintptr_t)weight % 4)
         return fail(NOP_E_ALIGNMENT, "a pointer is not aligned to its type");
-    int sms = 148;
-    if ((rc = rms::device_sms(&sms)) != NOP_OK) return rc;
+    int dev = 0, sms = 148;
+    if ((rc = current_device(&dev, &sms)) != NOP_OK) return rc;
     const rms::Cut c = rms::cut_of(*d, size, rms::on_16({x, residual, y, r, q}), sms, false);
     if (ceil_div(c.tiles, c.warps / c.W) > 0x7fffffffLL) return fail(NOP_E_UNSUPPORTED, "too many points");
     rms::Args a{};
@@ -612,8 +605,8 @@ int32_t nop_rms_norm_backward(const nop_norm_desc* d, const void* r, const float
     if (((uintptr_t)r | (uintptr_t)gy | (uintptr_t)gr | (uintptr_t)gx) % size || (uintptr_t)gw % 4 ||
         (uintptr_t)weight % 4 || (uintptr_t)workspace % 4)
         return fail(NOP_E_ALIGNMENT, "a pointer is not aligned to its type");
-    int sms = 148;
-    if ((rc = rms::device_sms(&sms)) != NOP_OK) return rc;
+    int dev = 0, sms = 148;
+    if ((rc = current_device(&dev, &sms)) != NOP_OK) return rc;
     const rms::Cut c = rms::cut_of(*d, size, rms::on_16({r, gy, gr, gx}), sms, true);
     const int slots = c.warps / c.W;
     int64_t grid = ceil_div(c.tiles, slots);
@@ -635,7 +628,7 @@ int32_t nop_rms_norm_backward(const nop_norm_desc* d, const void* r, const float
     a.tiles = c.tiles;
     a.eps = d->eps;
     rc = rms::dispatch<true>(d->dtype, c, [&](auto t, auto v, auto nc) {
-        return rms::launch_bwd<decltype(t), decltype(v)::value, decltype(nc)::value>(a, c, (unsigned)grid, s);
+        return rms::launch_bwd<decltype(t), decltype(v)::value, decltype(nc)::value>(a, c, (unsigned)grid, dev, s);
     });
     if (rc != NOP_OK || !gw) return rc;
     rms::k_reduce<<<d->channels, 128, 0, s>>>(a.partial, (int)rows, gw);
