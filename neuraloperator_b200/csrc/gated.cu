@@ -16,7 +16,8 @@
 // and after a tile's last chunk D2 goes out.  Two D1 buffers alternate, so the tensor core works on job k + 1's
 // first product while the epilogue warps work on job k; a tile's D2 is read after the next tile's first middle.
 //
-// Operands.  16-bit fields multiply as they are (products exact, fp32 sums).  fp32 values are split into three
+// Operands.  16-bit fields multiply as they are (products exact, fp32 sums); h, dg and du go into their products in two
+// 16-bit parts (Mid), and into the weights' gradients rounded once.  fp32 values are split into three
 // bf16 parts, v = a + b + c to within 2^-26 |v|, and six of the nine products are summed (the three left out are
 // below 2^-26): fp32 accuracy at the cost of six 16-bit MMAs, the same tensor time as three tf32 passes on a
 // hi / lo split but three quarters of its shared memory, and 2^-26 instead of 2^-21.  The tensor core adds to its
@@ -252,6 +253,30 @@ template <> __device__ __forceinline__ void images<float>(float2 v, uint32_t (&w
         w[i] = tc::pack_bf16(v.x, v.y);
         if (i < 2) v = __ffma2_rn(make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)),
                                   make_float2(-1.f, -1.f), v);
+    }
+}
+
+// The second product's A operand, which the middle makes from fp32 values: the three parts of fp32, and for a 16-bit
+// type the rounded value and the rounding of what is left.  With one rounding of h the output was off by up to 1.5
+// times its own rounding; the second MMA a step costs nothing that shows, the middle being the longer part.
+template <class T> struct Mid {
+    static constexpr int N = 2;
+};
+template <> struct Mid<float> {
+    static constexpr int N = 3;
+};
+template <class T> __device__ __forceinline__ void mid_images(float2 v, uint32_t (&w)[Mid<T>::N]) {
+    if constexpr (std::is_same<T, float>::value) {
+        images<T>(v, w);
+    } else {
+        uint32_t t[1];
+        images<T>(v, t);
+        w[0] = t[0];
+        float2 back;
+        if constexpr (std::is_same<T, __half>::value) back = __half22float2(*reinterpret_cast<const __half2*>(&t[0]));
+        else back = make_float2(__uint_as_float(t[0] << 16), __uint_as_float(t[0] & 0xFFFF0000u));
+        images<T>(__ffma2_rn(back, make_float2(-1.f, -1.f), v), t);
+        w[1] = t[0];
     }
 }
 
@@ -591,7 +616,7 @@ __global__ void __launch_bounds__(Roles<BWD>::THREADS, 1)
 k_block(const __grid_constant__ Params p, int* __restrict__ status) {
     constexpr int kEpi = Roles<BWD>::EPI, kMma = Roles<BWD>::MMA, kLoad = Roles<BWD>::LOAD;
     constexpr int kThreads = Roles<BWD>::THREADS, kGroups = Roles<BWD>::GROUPS;
-    constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N;
+    constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N, MID = Mid<T>::N;
     extern __shared__ __align__(1024) char sm[];
     const Plan& pl = p.pl;
     Bars& bar = *reinterpret_cast<Bars*>(sm + pl.o_bar);
@@ -868,7 +893,7 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
             };
             // ... x A images in tensor memory; image s of the K step of hidden group g at column col[s] + 16 g; the
             // smaller products in the N columns after D's
-            auto product_ts = [&](uint32_t d, const uint32_t (&col)[SPL], uint32_t bt, int N, int pw, bool acc, int g0) {
+            auto product_ts = [&](uint32_t d, const uint32_t (&col)[MID], uint32_t bt, int N, int pw, bool acc, int g0) {
                 uint64_t db[SPL];
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) db[s] = desc_of(bt + s * N * pw * 2, 256);
@@ -877,9 +902,13 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                 for (int ks = 0; ks < KC / 16; ++ks) {
                     if (ks >= pw / 16) break;
 #pragma unroll
-                    for (int i = 0; i < NP; ++i)
-                        mma_ts(i ? d + N : d, col[Passes<SPL>::a(i)] + 16 * (g0 + ks), db[Passes<SPL>::b(i)] + ks * bstep,
-                               id_2, i > 1 || acc || ks > 0, leader);
+                    for (int i = 0; i < (SPL == 1 ? MID : NP); ++i) {
+                        if constexpr (SPL == 1)
+                            mma_ts(d, col[i] + 16 * (g0 + ks), db[0] + ks * bstep, id_2, i > 0 || acc || ks > 0, leader);
+                        else
+                            mma_ts(i ? d + N : d, col[Passes<SPL>::a(i)] + 16 * (g0 + ks),
+                                   db[Passes<SPL>::b(i)] + ks * bstep, id_2, i > 1 || acc || ks > 0, leader);
+                    }
                 }
             };
             int j1 = 0, j2 = 0, k2 = 0;    // chunk of the first and of the second product, tile of the second
@@ -928,9 +957,10 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                     int at = j2 * pl.job_bytes + pl.NH * (2 * pl.Kx + pl.Ky) * 2 * SPL;
 #pragma unroll
                     for (int m = 0; m < (BWD ? 2 : 1); ++m) {
-                        uint32_t col[SPL];  // the places that the middle gave the images
+                        uint32_t col[MID];  // the places that the middle gave the images
                         if constexpr (SPL == 1) {
                             col[0] = d + m * pl.NH;
+                            col[1] = col[0] + 8;
                         } else {
                             col[0] = m ? d + pl.NH + 8 : d;
                             col[1] = m ? d + 2 * pl.NH : d + 8;
@@ -998,20 +1028,18 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                     u2[2 * i + 1] = __ffma2_rn(make_float2(vu[4 * i + 2], vu[4 * i + 3]), both(sc), make_float2(c.z, c.w));
                 }
                 if constexpr (!BWD) {
-                    uint32_t w[SPL][8];
+                    uint32_t w[MID][8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         float2 slope;
-                        uint32_t t[SPL];
-                        images<T>(__fmul2_rn(activation<GELU>(g2[i], slope), u2[i]), t);
+                        uint32_t t[MID];
+                        mid_images<T>(__fmul2_rn(activation<GELU>(g2[i], slope), u2[i]), t);
 #pragma unroll
-                        for (int s = 0; s < SPL; ++s) w[s][i] = t[s];
+                        for (int s = 0; s < MID; ++s) w[s][i] = t[s];
                     }
                     st8(d + 16 * g, w[0]);
-                    if constexpr (SPL == 3) {
-                        st8(d + 16 * g + 8, w[1]);
-                        st8(d + pl.NH + 16 * g, w[2]);
-                    }
+                    st8(d + 16 * g + 8, w[1]);
+                    if constexpr (SPL == 3) st8(d + pl.NH + 16 * g, w[MID - 1]);
                 } else {
                     float vf[16];
                     ld16(d + 2 * pl.NH + 16 * g, vf);
@@ -1019,7 +1047,7 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                     T* z = static_cast<T*>(p.z) + ((int64_t)(tile - p.tile0) * p.z_rows + h0) * TP + row;
                     T *zu = z + pl.H * TP, *zh = zu + pl.H * TP;
                     const int left = p.z ? pl.H - h0 : 0;
-                    uint32_t w[2][SPL][8];
+                    uint32_t w[2][MID][8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         float2 slope;
@@ -1028,11 +1056,11 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                         const float2 f = valid ? make_float2(vf[2 * i], vf[2 * i + 1]) : both(0.f);
                         const float2 h = valid ? __fmul2_rn(a, u2[i]) : both(0.f);
                         const float2 dg = __fmul2_rn(__fmul2_rn(f, u2[i]), slope), du = __fmul2_rn(f, a);
-                        uint32_t t[SPL], r[SPL];
-                        images<T>(dg, t);
-                        images<T>(du, r);
+                        uint32_t t[MID], r[MID];
+                        mid_images<T>(dg, t);
+                        mid_images<T>(du, r);
 #pragma unroll
-                        for (int s = 0; s < SPL; ++s) {
+                        for (int s = 0; s < MID; ++s) {
                             w[0][s][i] = t[s];
                             w[1][s][i] = r[s];
                         }
@@ -1057,7 +1085,9 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                     }
                     if constexpr (SPL == 1) {
                         st8(d + 16 * g, w[0][0]);
+                        st8(d + 16 * g + 8, w[0][1]);
                         st8(d + pl.NH + 16 * g, w[1][0]);
+                        st8(d + pl.NH + 16 * g + 8, w[1][1]);
                     } else {
                         st8(d + 16 * g, w[0][0]);
                         st8(d + 16 * g + 8, w[0][1]);
