@@ -11,6 +11,7 @@
 // partial sums up themselves, each in the same order, so there is no launch between the two, no atomic, and the
 // result does not depend on scheduling.  The scaling walks the chunks backwards: the last chunks that the norm
 // read are still in the 126 MB L2.
+#include "l2_hints.cuh"
 #include "nop_internal.cuh"
 
 #include <cuda_fp16.h>
@@ -37,6 +38,7 @@ namespace clip {
 constexpr int kItems = 256;         // tensors a launch (a 32-byte entry each in the kernel parameters)
 constexpr int kChunk = 8192;        // values a chunk
 constexpr int kThreads = 256;
+constexpr uint32_t kKeep = 2560;    // chunks of a launch that L2 is asked to keep for the scaling: 80 MB in fp32
 constexpr int kMaxGrid = 1024;      // partial sums a launch leaves at most
 
 struct Item {
@@ -103,7 +105,7 @@ __device__ double block_join(double v) {
 // A thread's part of one chunk: at most kChunk / kThreads = 32 squares in fp32 before they join the running
 // sum in 64 bits, so the sum over any number of values keeps fp32's precision.
 template <bool INF, class T>
-__device__ float chunk_value(const T* __restrict__ src, int len) {
+__device__ float chunk_value(const T* __restrict__ src, int len, uint64_t pol) {
     float s = 0.f;
     constexpr int V = 16 / (int)sizeof(T);
     if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
@@ -111,7 +113,7 @@ __device__ float chunk_value(const T* __restrict__ src, int len) {
         const int nv = len / V;
 #pragma unroll 4
         for (int i = threadIdx.x; i < nv; i += kThreads) {
-            const uint4 q = __ldg(v4 + i);
+            const float4 q = l2::ld4(v4 + i, pol);
             const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
             for (int j = 0; j < V; ++j) s = add_value<INF>(s, to_f(e[j]));
@@ -126,15 +128,17 @@ __device__ float chunk_value(const T* __restrict__ src, int len) {
 
 template <bool INF>
 __global__ void __launch_bounds__(kThreads) k_norm(const __grid_constant__ Table t, double* __restrict__ partial) {
+    const uint64_t keep = l2::evict_last(), pass = l2::evict_first();
     double acc = 0.0;
     for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const Item& it = item_of(t, c);
         const int64_t at = (int64_t)(c - it.first) * kChunk;
         const int len = (int)(it.n - at < kChunk ? it.n - at : kChunk);
+        const uint64_t pol = t.chunks - c <= kKeep ? keep : pass;
         float s;
-        if (it.dtype == NOP_DTYPE_FP32) s = chunk_value<INF>(static_cast<const float*>(it.src) + at, len);
-        else if (it.dtype == NOP_DTYPE_BF16) s = chunk_value<INF>(static_cast<const __nv_bfloat16*>(it.src) + at, len);
-        else s = chunk_value<INF>(static_cast<const __half*>(it.src) + at, len);
+        if (it.dtype == NOP_DTYPE_FP32) s = chunk_value<INF>(static_cast<const float*>(it.src) + at, len, pol);
+        else if (it.dtype == NOP_DTYPE_BF16) s = chunk_value<INF>(static_cast<const __nv_bfloat16*>(it.src) + at, len, pol);
+        else s = chunk_value<INF>(static_cast<const __half*>(it.src) + at, len, pol);
         acc = join<INF>(acc, (double)s);
     }
     acc = block_join<INF>(acc);

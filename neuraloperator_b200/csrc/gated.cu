@@ -84,11 +84,12 @@ template <int SPL> struct Passes {
     __device__ static constexpr int b(int i) { return i == 1 || i == 3 ? 1 : i == 4 ? 2 : 0; }
 };
 
-// Warps of k_block: the middle's (and output's), the producers' (in groups of four that take the pieces in turn), MMA
-// issue, weight copies.
-template <bool BWD> struct Roles {
-    static constexpr int EPI = 8, GROUPS = BWD ? 1 : 2, MMA = EPI + 4 * GROUPS, LOAD = MMA + 1, THREADS = 32 * (LOAD + 1);
-};
+// Warps of k_block.
+constexpr int kEpi = 8;                       // 0..7: middle and output
+constexpr int kProd = 4;                      // 8..11: x (and e) into shared memory
+constexpr int kMma = kEpi + kProd;            // 12: MMA issue
+constexpr int kLoad = kMma + 1;               // 13: weight copies
+constexpr int kThreads = 32 * (kLoad + 1);    // 14 warps: 128 registers a thread
 
 struct Plan {
     int C, H, O;               // channels of x, hidden width, channels of y
@@ -612,10 +613,8 @@ struct Bars {
 };
 
 template <class T, class IN, bool BWD, bool GELU>
-__global__ void __launch_bounds__(Roles<BWD>::THREADS, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 k_block(const __grid_constant__ Params p, int* __restrict__ status) {
-    constexpr int kEpi = Roles<BWD>::EPI, kMma = Roles<BWD>::MMA, kLoad = Roles<BWD>::LOAD;
-    constexpr int kThreads = Roles<BWD>::THREADS, kGroups = Roles<BWD>::GROUPS;
     constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N, MID = Mid<T>::N;
     extern __shared__ __align__(1024) char sm[];
     const Plan& pl = p.pl;
@@ -625,7 +624,7 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
         for (int i = 0; i < kMaxA; ++i) {
-            tc::mbar_init(&bar.full_a[i], 4);
+            tc::mbar_init(&bar.full_a[i], kProd);
             tc::mbar_init(&bar.empty_a[i], 1);
         }
         for (int i = 0; i < kMaxB; ++i) {
@@ -683,10 +682,10 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
     if (warp >= kEpi && warp < kMma) {
         // ------------------------------ x / e -> shared memory ------------------------------
         // a warp takes the 16-byte columns w, w + 4 of every piece; x and e have the same type in the backward
-        const int w = (warp - kEpi) & 3, group = (warp - kEpi) >> 2;
+        const int w = warp - kEpi;
         constexpr int NI = KC / 32;                       // items a thread has in a piece
         const int total = (pl.reuse ? my : jobs) * nA;
-        // The group's place in the sequence of pieces (tile k, chunk j, piece kc), for the loads and for the stores,
+        // The place in the sequence of pieces (tile k, chunk j, piece kc), for the loads and for the stores,
         // which run one piece behind; the slot and its phase go with the stores.
         struct Place {
             int k, j, kc, i;
@@ -703,12 +702,11 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
         auto advance = [&](Place& q) {
             if (++q.i < units) return;
             q.i = 0;
-            for (q.kc += kGroups; q.kc >= nA;) {
-                q.kc -= nA;
-                if (++q.j == chunks) {
-                    q.j = 0;
-                    ++q.k;
-                }
+            if (++q.kc < nA) return;
+            q.kc = 0;
+            if (++q.j == chunks) {
+                q.j = 0;
+                ++q.k;
             }
         };
         auto load = [&](Flight& f, Place& q) {
@@ -732,8 +730,8 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
             }
             advance(q);
         };
-        int slot = group % pl.na;
-        uint32_t phase = 1 ^ ((group / pl.na) & 1);       // of the slot's last release: none is needed the first time
+        int slot = 0;
+        uint32_t phase = 1;       // of the slot's last release: none is needed the first time
         auto put = [&](const Flight& f, Place& q) -> bool {
             if (q.k >= my) return false;
             const bool is_x = !BWD || q.kc < pl.nKx;
@@ -779,19 +777,17 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&bar.full_a[slot]);
-                for (slot += kGroups; slot >= pl.na;) {
-                    slot -= pl.na;
+                if (++slot == pl.na) {
+                    slot = 0;
                     phase ^= 1;
                 }
             }
             advance(q);
             return true;
         };
-        // the group's next piece is in flight while this one waits for its slot and is written
+        // the next piece is in flight while this one waits for its slot and is written
         Flight c, d;
-        Place in{0, 0, group - kGroups, units - 1}, at;
-        advance(in);
-        at = in;
+        Place in{0, 0, 0, 0}, at = in;
         load(c, in);
         while (true) {
             load(d, in);
@@ -1744,8 +1740,8 @@ int32_t forward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, co
         q.out = o.y;
         q.vec = d.points % 4 == 0 && aligned({o.x}, 4 * sizeof(IN));
         rc = d.activation == NOP_ACT_GELU
-                 ? launch<k_block<T, IN, false, true>>(dev, grid, Roles<false>::THREADS, p.smem, s, q, dev.status)
-                 : launch<k_block<T, IN, false, false>>(dev, grid, Roles<false>::THREADS, p.smem, s, q, dev.status);
+                 ? launch<k_block<T, IN, false, true>>(dev, grid, kThreads, p.smem, s, q, dev.status)
+                 : launch<k_block<T, IN, false, false>>(dev, grid, kThreads, p.smem, s, q, dev.status);
         if (rc != NOP_OK || p.col0 + p.cols >= p.O) return rc;
         if (!make_plan<T>(d, false, p.col0 + p.cols, &p)) return fail(NOP_E_UNSUPPORTED, kTooLarge);
     }
@@ -1799,8 +1795,8 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
         q.tile0 = (int)t;
         q.tiles = (int)std::min<int64_t>(slab, z.tiles - t);
         const unsigned grid = (unsigned)std::min<int64_t>(q.tiles, dev.sms);
-        rc = d.activation == NOP_ACT_GELU ? launch<k_block<T, T, true, true>>(dev, grid, Roles<true>::THREADS, p.smem, s, q, dev.status)
-                                          : launch<k_block<T, T, true, false>>(dev, grid, Roles<true>::THREADS, p.smem, s, q, dev.status);
+        rc = d.activation == NOP_ACT_GELU ? launch<k_block<T, T, true, true>>(dev, grid, kThreads, p.smem, s, q, dev.status)
+                                          : launch<k_block<T, T, true, false>>(dev, grid, kThreads, p.smem, s, q, dev.status);
         if (rc != NOP_OK) return rc;
         if (!weights) continue;
         w.pieces = q.tiles * (TP / WForm<T>::KC);
@@ -1818,8 +1814,8 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
         r.out = q.out;
         r.vec = q.vec;
         const unsigned grid = (unsigned)std::min<int64_t>(z.tiles, dev.sms);
-        rc = d.activation == NOP_ACT_GELU ? launch<k_block<T, T, true, true>>(dev, grid, Roles<true>::THREADS, p.smem, s, r, dev.status)
-                                          : launch<k_block<T, T, true, false>>(dev, grid, Roles<true>::THREADS, p.smem, s, r, dev.status);
+        rc = d.activation == NOP_ACT_GELU ? launch<k_block<T, T, true, true>>(dev, grid, kThreads, p.smem, s, r, dev.status)
+                                          : launch<k_block<T, T, true, false>>(dev, grid, kThreads, p.smem, s, r, dev.status);
         if (rc != NOP_OK) return rc;
     }
     if (!weights) return NOP_OK;
