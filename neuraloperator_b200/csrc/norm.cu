@@ -17,6 +17,11 @@
 // channels of the same points: warp k holds channels k, k + W, ... (at most NC) in registers between the sums
 // and the scaling, and the W partial sums meet in shared memory.  More than 256 channels do not fit the
 // registers of a CTA: the second pass then reads the tile again, out of L2.
+//
+// Measured on B200, 64 channels x 2^21 points fp32, of the measured copy bandwidth: forward 193 us (86%), with the
+// residual 342 us (97%), backward 406 us (61%) and 442 us with the residual's gradient (75%; two fields in registers and
+// a meeting of the warps between them and the output).  Rows that are not aligned load one value a thread: 55 to 80% in
+// fp32, 25 to 40% in bf16, whose two-byte loads keep too few bytes in flight.
 #include "nop_internal.cuh"
 
 #include <cuda_fp16.h>
