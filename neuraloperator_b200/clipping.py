@@ -84,7 +84,8 @@ def clip_by_global_norm(tensors: Iterable[torch.Tensor], max_norm: float,
     if not tensors:
         return [], torch.zeros(())
     dev = _check(tensors)
-    src = [t if t.is_contiguous() and not t.is_conj() else t.resolve_conj().contiguous() for t in tensors]
+    src = [t if t.is_contiguous() and not t.is_conj() and not t.is_neg()
+           else t.resolve_conj().resolve_neg().contiguous() for t in tensors]
     dst = [torch.empty_like(t) for t in src]
     return dst, _run(src, dst, limit, kind, dev)
 
@@ -110,7 +111,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
             raise RuntimeError(f"the total norm of the gradients is {float(norm)}, so it cannot be clipped; pass "
                                "error_if_nonfinite=False to scale by it anyway")
     norm = _run(flat, flat, limit, kind, dev)
-    torch.autograd.graph.increment_version(flat)  # written behind autograd's back
+    torch.autograd.graph.increment_version([t for t in flat if not t.is_inference()])  # written behind autograd's back
     for g, f in zip(grads, flat):
         if f is not g:
             g.copy_(f)

@@ -134,7 +134,8 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     """y [batch, out, *grid] (see the module docstring).  x: a field [batch, channels, *grid] on a CUDA device;
     w_gate, w_up: [hidden, channels], w_down: [out, hidden] (or Conv1d weights [., ., 1]); biases [hidden], [hidden],
     [out] or None; all of x's dtype: float32 (fp32 accuracy), bfloat16 or float16 (fp32 sums).  activation: "silu" or
-    "gelu" (exact).  channels and out <= 256, hidden <= 16384.
+    "gelu" (exact).  channels and out <= 256, hidden <= 16384.  The hidden values have the dtype's range (float16: a
+    hidden value above 65504 makes its point's output not finite).
 
     With ``x_scale`` (float32 [batch, 1, *grid]) x is float8_e4m3fn and stands for x * x_scale, as
     ``rms_norm_quantized`` leaves it; weights and output are bfloat16 or float16 (inference only).

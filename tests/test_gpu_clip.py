@@ -173,3 +173,18 @@ def test_training_step_of_a_model():
     assert abs(float(norm) - n) <= n * 20 * V
     for p, b in zip(model.parameters(), before):
         check_scaled([p.grad], [b], 0.1)
+
+
+def test_lazy_views_and_inference_tensors():
+    z = make((9, 4), torch.complex64, 5)
+    neg = torch._neg_view(make((50,), torch.float32, 6))  # contiguous, its sign only noted
+    n = norm64([z, neg])
+    out, _ = nb.clip_by_global_norm([z.conj(), neg], n / 2)
+    check_scaled([out[0]], [z.conj().resolve_conj()], 0.5)
+    check_scaled([out[1]], [neg.resolve_neg()], 0.5)
+    with torch.inference_mode():
+        p = torch.nn.Parameter(make((100,), torch.float32, 1), requires_grad=False)
+        p.grad = make((100,), torch.float32, 2)
+        kept = p.grad.clone()
+        nb.clip_grad_norm_(p, float(kept.norm()) / 2)
+        check_scaled([p.grad], [kept], 0.5)

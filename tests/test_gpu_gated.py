@@ -299,3 +299,24 @@ def test_norm_block_and_clipping_together():
     assert abs(float(norm) - n) <= 4e-6 * n
     for p, g in zip(ours, grads):
         assert rel(p.grad, g * 0.01 / n) <= 4e-6
+
+
+def test_offsets_past_32_bits():
+    """A field of 2.2e9 values: its last points, forward, backward and both kinds of rows, equal those of a small one."""
+    c, h, o = 256, 20, 3
+    rest = operands(1, c, h, o, (1,), torch.bfloat16, seed=3)[1:]
+    for p in (4_300_000, 4_300_001):
+        x = torch.zeros(2, c, p, device="cuda", dtype=torch.bfloat16)
+        gy = torch.zeros(2, o, p, device="cuda", dtype=torch.bfloat16)
+        n = 2 * p % 128 + 128   # the last tiles, whole: a small field of them has the same tiles
+        x[1, :, p - n:], gy[1, :, p - n:] = make((c, n), torch.bfloat16, 1), make((o, n), torch.bfloat16, 2)
+        x.requires_grad_()
+        y = nb.gated_mlp(x, *rest)
+        (gx,) = torch.autograd.grad(y, x, gy)
+        xs = x.detach()[1:, :, p - n:].clone().requires_grad_()
+        ys = nb.gated_mlp(xs, *rest)
+        (gs,) = torch.autograd.grad(ys, xs, gy[1:, :, p - n:].contiguous())
+        assert torch.equal(y[1:, :, p - n:], ys) and torch.equal(gx[1:, :, p - n:], gs)
+        assert (gx[:, :, : p - n] == 0).all()
+        assert _lib.device_status() == 0
+        del x, y, gx

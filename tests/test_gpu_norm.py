@@ -229,3 +229,25 @@ def test_captured_and_replayed():
         kept = [t.clone() for t in out]
         for a, b in zip(kept, step()):
             assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    """A field of 2.2e9 values: the last points of the last channel, forward and backward."""
+    c, p = 32, 70_000_003
+    x = torch.zeros(1, c, p, device="cuda", dtype=torch.bfloat16)
+    tail = slice(p - 300, p)
+    x[..., tail] = make((1, c, 300), torch.bfloat16, 1)
+    w = make((c,), torch.float32, 2)
+    with torch.no_grad():
+        y = nb.rms_norm(x, w, eps=EPS)
+    y64, _, inv = define(x[..., tail], w, None)
+    assert ((y[..., tail].double() - y64).abs() <= y_bound(y64, c, torch.bfloat16)).all()
+    assert (y[..., : p - 300] == 0).all()
+    del y
+    x.requires_grad_()
+    g = torch.zeros_like(x, requires_grad=False)
+    g[..., tail] = make((1, c, 300), torch.bfloat16, 3)
+    (gx,) = torch.autograd.grad(nb.rms_norm(x, w, eps=EPS), x, g)
+    xs = x.detach()[..., tail].clone().requires_grad_()
+    (want,) = torch.autograd.grad(nb.rms_norm(xs, w, eps=EPS), xs, g[..., tail].contiguous())
+    assert torch.equal(gx[..., tail], want)
