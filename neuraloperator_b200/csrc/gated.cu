@@ -13,8 +13,8 @@
 //   middle          the epilogue warps read D1, apply the activation and write h (backward: dg, du) back into the
 //                   same columns of tensor memory as the next A operand -- h never leaves the SM in the forward
 //   second product  D2 += h W_down^T (backward: dg W_gate + du W_up), A from tensor memory
-// and after a tile's last chunk D2 goes out.  Two D1 buffers alternate, so the tensor core works on job k + 1's
-// first product while the epilogue warps work on job k; a tile's D2 is read after the next tile's first middle.
+// and after a tile's last chunk D2 goes out.  Two or three D1 buffers take turns, so the tensor core works on the next
+// jobs' first products while the epilogue warps work on a job; a tile's D2 is read after the next tile's first middle.
 //
 // Operands.  16-bit fields multiply as they are (products exact, fp32 sums); h, dg and du go into their products in two
 // 16-bit parts (Mid), and into the weights' gradients rounded once.  fp32 values are split into three
@@ -104,7 +104,7 @@ struct Plan {
     int Kx, Ky;                // padded K of the first products (Ky: backward only, 0 otherwise)
     int cols, col0;            // channels of this launch's output, the first of them
     int N2;                    // padded columns of D2
-    int n_d2;                  // D2 buffers
+    int n_d1, n_d2;            // D1 buffers (jobs in flight), D2 buffers
     int NH, nJ;                // chunk width, chunks
     int nKx, nKy, nH;          // ring pieces: of x, of e, of a chunk in the second product
     int na, nb;                // ring slots (nb: streaming)
@@ -615,7 +615,7 @@ __device__ __forceinline__ void copy_item(const Item<T>& it, T* __restrict__ z, 
 // barriers, by index into the barrier area
 struct Bars {
     uint64_t full_a[kMaxA], empty_a[kMaxA], full_b[kMaxB], empty_b[kMaxB];
-    uint64_t d1[2], mid[2], g2[2], d2[2], d2_free[2], drain;
+    uint64_t d1[3], mid[3], g2[3], d2[2], d2_free[2], drain;
     uint32_t tmem;
     int abort_flag;
 };
@@ -639,10 +639,12 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
             tc::mbar_init(&bar.full_b[i], 1);
             tc::mbar_init(&bar.empty_b[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 3; ++i) {
             tc::mbar_init(&bar.d1[i], 1);
             tc::mbar_init(&bar.mid[i], kEpi);
             tc::mbar_init(&bar.g2[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&bar.d2[i], 1);
             tc::mbar_init(&bar.d2_free[i], kEpi);
         }
@@ -681,7 +683,8 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
     const int nA = pl.nKx + pl.nKy;                       // A pieces of a job
     const int d1w = (BWD ? 3 : 2) * pl.NH;                // columns of a D1 buffer
     const int d2w = pl.N2 * (SPL == 3 ? 2 : 1);           // columns of a D2 buffer (D2c after D2)
-    const uint32_t d2_0 = tmem + 2 * d1w;
+    const uint32_t d2_0 = tmem + pl.n_d1 * d1w;
+    const int lead = pl.n_d1 - 1;                         // first products run so many jobs ahead of second ones
     // D2 buffer of this CTA's tile k, and how often it was used before
     auto d2_buf = [&](int k) { return pl.n_d2 == 2 ? k & 1 : 0; };
     auto d2_use = [&](int k) { return pl.n_d2 == 2 ? k >> 1 : k; };
@@ -823,14 +826,14 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                     ++q;
                     return bytes;
                 };
-                for (int J = 0; J <= jobs && ok; ++J) {  // in the order of the MMA warp
+                for (int J = 0; J < jobs + lead && ok; ++J) {  // in the order of the MMA warp
                     if (J < jobs) {
                         const char* src = p.packed + (int64_t)(J % pl.nJ) * pl.job_bytes;
                         for (int kc = 0; kc < pl.nKx && ok; ++kc) src += push(src, 2 * pl.NH, piece_k(pl.Kx, KC, kc));
                         for (int kc = 0; kc < pl.nKy && ok; ++kc) src += push(src, pl.NH, piece_k(pl.Ky, KC, kc));
                     }
-                    if (J > 0 && ok) {
-                        const char* src = p.packed + (int64_t)((J - 1) % pl.nJ) * pl.job_bytes +
+                    if (J >= lead && ok) {
+                        const char* src = p.packed + (int64_t)((J - lead) % pl.nJ) * pl.job_bytes +
                                           (int64_t)pl.NH * (2 * pl.Kx + pl.Ky) * 2 * SPL;
                         for (int m = 0; m < (BWD ? 2 : 1); ++m)
                             for (int kc = 0; kc < pl.nH && ok; ++kc) src += push(src, pl.N2, piece_k(pl.NH, KC, kc));
@@ -916,12 +919,13 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                 }
             };
             int j1 = 0, j2 = 0, k2 = 0;    // chunk of the first and of the second product, tile of the second
-            for (int J = 0; J <= jobs && ok; ++J) {
-                const int b = J & 1;
+            int b1 = 0, b2 = 0;            // D1 buffers of the two
+            uint32_t p1 = 1, p2 = 0;       // phases: of the first one's last second product, of the second one's middle
+            for (int J = 0; J < jobs + lead && ok; ++J) {
                 if (J < jobs) {  // first product of job J
-                    if (J >= 2 && !all(&bar.g2[b], (uint32_t)((J >> 1) - 1) & 1)) break;
+                    if (!all(&bar.g2[b1], p1)) break;  // (true of a new barrier's phase 1)
                     fence_after();
-                    const uint32_t d = tmem + b * d1w;
+                    const uint32_t d = tmem + b1 * d1w;
                     const bool last = j1 == pl.nJ - 1;
                     int at = j1 * pl.job_bytes, slot = a0;
                     uint32_t phase = ap;
@@ -944,20 +948,24 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                         }
                     }
                     if (!ok) break;
-                    commit(&bar.d1[b], leader);
+                    commit(&bar.d1[b1], leader);
+                    if (++b1 == pl.n_d1) {
+                        b1 = 0;
+                        p1 ^= 1;
+                    }
                     if (!pl.reuse || last) {
                         a0 = slot;
                         ap = phase;
                     }
                     j1 = last ? 0 : j1 + 1;
                 }
-                if (J > 0) {  // second product of job J - 1
-                    if (!all(&bar.mid[b ^ 1], (uint32_t)((J - 1) >> 1) & 1)) break;
+                if (J >= lead) {  // second product of job J - lead
+                    if (!all(&bar.mid[b2], p2)) break;
                     const int e = d2_buf(k2);
                     if (j2 == 0 && d2_use(k2) > 0 && !all(&bar.d2_free[e], (uint32_t)(d2_use(k2) - 1) & 1)) break;
                     const uint32_t d2 = d2_0 + e * d2w;
                     fence_after();
-                    const uint32_t d = tmem + (b ^ 1) * d1w;
+                    const uint32_t d = tmem + b2 * d1w;
                     int at = j2 * pl.job_bytes + pl.NH * (2 * pl.Kx + pl.Ky) * 2 * SPL;
 #pragma unroll
                     for (int m = 0; m < (BWD ? 2 : 1); ++m) {
@@ -981,7 +989,11 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                         }
                     }
                     if (!ok) break;
-                    commit(&bar.g2[b ^ 1], leader);
+                    commit(&bar.g2[b2], leader);
+                    if (++b2 == pl.n_d1) {
+                        b2 = 0;
+                        p2 ^= 1;
+                    }
                     if (++j2 == pl.nJ) {
                         commit(&bar.d2[e], leader);
                         j2 = 0;
@@ -1000,13 +1012,14 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const int groups = pl.NH / 16;
 
-        auto middle = [&](int J, int k, int j) -> bool {
-            const int b = J & 1;
+        int b = 0;                 // D1 buffer and its phase
+        uint32_t phase = 0;
+        auto middle = [&](int k, int j) -> bool {
             const uint32_t tile = tile_at(k), n = tile * TP + row;
             const bool valid = n < p.points;
             float sc = 1.f;
             if constexpr (sizeof(IN) == 1) sc = valid ? __ldg(p.scale + n) : 0.f;
-            if (!wait(&bar.d1[b], (uint32_t)(J >> 1) & 1)) return false;
+            if (!wait(&bar.d1[b], phase)) return false;
             fence_after();
             const uint32_t d = tmem + b * d1w + lanes;
             for (int g = part; g < groups; g += kEpi / 4) {
@@ -1106,6 +1119,10 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
             fence_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&bar.mid[b]);
+            if (++b == pl.n_d1) {
+                b = 0;
+                phase ^= 1;
+            }
             return true;
         };
         auto output = [&](int k) -> bool {
@@ -1166,9 +1183,9 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
             return true;
         };
         bool ok = true;
-        for (int J = 0, k = 0; k < my && ok; ++k) {
-            for (int j = 0; j < pl.nJ && ok; ++j, ++J) {
-                ok = middle(J, k, j);
+        for (int k = 0; k < my && ok; ++k) {
+            for (int j = 0; j < pl.nJ && ok; ++j) {
+                ok = middle(k, j);
                 if (ok && j == 0 && k > 0) ok = output(k - 1);
             }
         }
@@ -1531,7 +1548,7 @@ k_finish(WParams p, T* __restrict__ gwg, T* __restrict__ gwu, T* __restrict__ gw
 // How a call is cut.  An fp32 launch takes at most 128 output channels (D2 and D2c); more are several launches, each
 // with the whole first product.  Tensor memory: two D1 buffers and D2 (fp32: and D2c) in 512 columns, so the
 // backward's chunk (three columns a hidden channel) is 64 wide when D2 takes up to 128 of them and 32 above; what is
-// left may hold a second D2.  Shared memory: the weights stay when they
+// left holds a third D1, or a second D2, or both.  Shared memory: the weights stay when they
 // leave room for two pieces of A, otherwise two to six pieces of each stream.
 template <class T>
 bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
@@ -1548,7 +1565,9 @@ bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
     const int most = bwd && p.N2 * (SPL == 3 ? 2 : 1) > 128 ? 32 : 64;
     p.nJ = (p.H + most - 1) / most;
     p.NH = up16((p.H + p.nJ - 1) / p.nJ);
-    p.n_d2 = 2 * (bwd ? 3 : 2) * p.NH + 2 * p.N2 * (SPL == 3 ? 2 : 1) <= 512 ? 2 : 1;
+    const int w1 = (bwd ? 3 : 2) * p.NH, w2 = p.N2 * (SPL == 3 ? 2 : 1);
+    p.n_d1 = 3 * w1 + w2 <= 512 ? 3 : 2;
+    p.n_d2 = p.n_d1 * w1 + 2 * w2 <= 512 ? 2 : 1;
     p.nKx = (p.Kx + KC - 1) / KC;
     p.nKy = (p.Ky + KC - 1) / KC;
     p.nH = (p.NH + KC - 1) / KC;
