@@ -42,13 +42,16 @@
 // epilogue warps add the accumulator (fp32: and the smaller products' own) to registers.
 // The scratch is made and consumed slab by slab.
 //
-// Measured on B200.  What bounds k_block is the chain of a job, first product -> middle -> second product, with two jobs
-// in flight: at fp32 64 / 128 / 64 (channels, hidden, out) the tensor pipe is active 55% of the time and 41% of the issue
-// slots are used.  The forward of 2^21 points takes 500 us (600 in a long run, at the power cap's 1.6 GHz), where the
-// bytes take 166 us and six 16-bit products 371 us at the measured peaks; bf16 128 / 384 / 128 on 32 fields of 85 x 85,
-// rows not aligned: 156 us forward, 482 us backward (products alone: 41 and 110 us).  k_wgrad moves 4.6 TB/s.  Pairs of
-// CTAs (cta_group::2, half of the weights in each) ran slower at nearly all sizes (fp32 forward above 548 us, bf16
-// 32 / 32 / 32 121 us against 70): the second CTA lengthens the chain by its arrivals.
+// Measured on B200.  fp32, 64 / 128 / 64 (channels, hidden, out): the forward of 2^21 points takes 500 us (600 in a long
+// run, at the power cap's 1.6 GHz), where the bytes take 166 us and six 16-bit products 371 us at the measured peaks.
+// It is bound by the MMA warp, which never waits: the first product's MMAs take 105 cycles each instead of the 68 of
+// their arithmetic, both operands coming from shared memory, the second one's (N = 64) 50; the middle takes 1650 cycles
+// of a job's 4050.  A third D1 buffer, more weights or pieces of x in flight, or MMAs issued in blocks changed nothing.
+// 16-bit types are bound by the middle (800 cycles for 16 hidden channels of a warp's points; exponentials, reciprocals
+// and conversions): bf16 128 / 384 / 128 on 32 fields of 85 x 85, rows not aligned, 150 us forward and 480 us backward
+// (products alone: 41 and 110 us).  In the backward the scratch's stores lengthen the middle to 4400 cycles a job, and
+// k_wgrad reads it at 4.6 TB/s.  Pairs of CTAs (cta_group::2, half of the weights in each) ran slower at nearly all
+// sizes (fp32 forward above 548 us, bf16 32 / 32 / 32 121 us against 70).
 //
 // Every wait is bounded: on expiry the kernel records NOP_DEVICE_MMA_TIMEOUT in the status word, all roles leave
 // their loops, copies and MMAs in flight are waited for (bounded) and the tensor memory is freed.
@@ -695,7 +698,6 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
         // a warp takes the 16-byte columns w, w + 4 of every piece; x and e have the same type in the backward
         const int w = warp - kEpi;
         constexpr int NI = KC / 32;                       // items a thread has in a piece
-        const int total = (pl.reuse ? my : jobs) * nA;
         // The place in the sequence of pieces (tile k, chunk j, piece kc), for the loads and for the stores,
         // which run one piece behind; the slot and its phase go with the stores.
         struct Place {
