@@ -589,6 +589,30 @@ __device__ __forceinline__ void store_rows(T* at, uint32_t two, int lane, int le
     if (left > (odd ? 1 : 0)) *reinterpret_cast<uint32_t*>(at + (odd ? TP - 1 : 0)) = word;
 }
 
+// the same rows in fp32
+__device__ __forceinline__ void store_wide(float* at, float2 v, int left) {
+    if (left > 0) at[0] = v.x;
+    if (left > 1) at[TP] = v.y;
+}
+
+// an item of a 16-bit field as rows of 128 points in fp32
+template <class T>
+__device__ __forceinline__ void copy_wide(const Item<T>& it, float* __restrict__ z, int c0, int rows, int lane) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (c0 + e >= rows) break;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint16_t h = (uint16_t)(it.w[2 * e + i / 2] >> (16 * (i & 1)));
+                v[i] = to_f(*reinterpret_cast<const T*>(&h));
+            }
+            *reinterpret_cast<float4*>(z + (c0 + e) * TP + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    }
+}
+
 // the item's channels below `rows` as rows of 128 points
 template <class T>
 __device__ __forceinline__ void copy_item(const Item<T>& it, T* __restrict__ z, int c0, int rows, int lane, bool vec) {
@@ -623,7 +647,8 @@ struct Bars {
     int abort_flag;
 };
 
-template <class T, class IN, bool BWD, bool GELU>
+// WIDE: the scratch is fp32 (of a 16-bit field with few points)
+template <class T, class IN, bool BWD, bool GELU, bool WIDE = false>
 __global__ void __launch_bounds__(kThreads, 1)
 k_block(const __grid_constant__ Params p, int* __restrict__ status) {
     constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N, MID = Mid<T>::N;
@@ -758,11 +783,12 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                 const int ch = w + 4 * i;
                 if (ch * 8 < pw) store_item<T, IN>(it, s, ch, pw / 16, lane, p.vec);
                 if constexpr (BWD) {
-                    if (keep)
-                        copy_item<T>(it,
-                                     static_cast<T*>(p.z) + ((int64_t)(tile_at(q.k) - p.tile0) * p.z_rows + 3 * pl.H +
-                                                             (is_x ? 0 : pl.C)) * TP,
-                                     c0 + ch * 8, is_x ? pl.C : pl.O, lane, p.vec);
+                    const int64_t to =
+                        ((int64_t)(tile_at(q.k) - p.tile0) * p.z_rows + 3 * pl.H + (is_x ? 0 : pl.C)) * TP;
+                    if (keep && WIDE)
+                        copy_wide<T>(it, static_cast<float*>(p.z) + to, c0 + ch * 8, is_x ? pl.C : pl.O, lane);
+                    else if (keep)
+                        copy_item<T>(it, static_cast<T*>(p.z) + to, c0 + ch * 8, is_x ? pl.C : pl.O, lane, p.vec);
                 }
             };
             Item<IN> it;
@@ -1063,7 +1089,9 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                     float vf[16];
                     ld16(d + 2 * pl.NH + 16 * g, vf);
                     wait_ld(vf);
-                    T* z = static_cast<T*>(p.z) + ((int64_t)(tile - p.tile0) * p.z_rows + h0) * TP + row;
+                    const int64_t z_at = ((int64_t)(tile - p.tile0) * p.z_rows + h0) * TP + row;
+                    T* z = static_cast<T*>(p.z) + z_at;
+                    float* zw = static_cast<float*>(p.z) + z_at;
                     T *zu = z + pl.H * TP, *zh = zu + pl.H * TP;
                     const int left = p.z ? pl.H - h0 : 0;
                     uint32_t w[2][MID][8];
@@ -1083,7 +1111,11 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                             w[0][s][i] = t[s];
                             w[1][s][i] = r[s];
                         }
-                        if constexpr (SPL == 1) {
+                        if constexpr (WIDE) {
+                            store_wide(zw + 2 * i * TP, dg, left - 2 * i);
+                            store_wide(zw + (pl.H + 2 * i) * TP, du, left - 2 * i);
+                            store_wide(zw + (2 * pl.H + 2 * i) * TP, h, left - 2 * i);
+                        } else if constexpr (SPL == 1) {
                             uint32_t o[1];
                             images<T>(h, o);
                             store_rows(z + 2 * i * TP, t[0], lane, left - 2 * i);
@@ -1615,7 +1647,13 @@ struct Sizes {
     size_t packed, vec, z, partial, sums, bytes;
     int64_t slab_tiles, tiles;
     int splits, wtiles;
+    bool wide;
 };
+
+// A 16-bit field's dg, du and h are rounded for the weights' gradients, by as much as the gradients are.  Over many
+// points that averages (1.4 times the result's own rounding); with few, an element could be off by twice it, and the
+// scratch is fp32, at a cost that is small there: the fp32 path of k_wgrad.
+constexpr int64_t kWidePoints = 1 << 15;
 
 template <class T>
 Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd) {
@@ -1636,11 +1674,12 @@ Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd) {
         // The scratch of a slab: up to 512 MB, in whole waves of 148 tiles.  Slabs that stay in L2 save the scratch's
         // trip through HBM but lose more to their launches' beginnings and ends: 64 MB slabs took 2207 us where
         // 512 MB take 1646 (fp32, 64 channels, hidden 128, 2^20 points), and larger ones 1626.
-        const int64_t tile_bytes = (int64_t)(3 * p.H + p.C + p.O) * TP * sizeof(T);
+        s.wide = sizeof(T) == 4 || s.tiles * TP <= kWidePoints;
+        const int64_t tile_bytes = (int64_t)(3 * p.H + p.C + p.O) * TP * (s.wide ? 4 : 2);
         const int64_t waves = std::max<int64_t>(1, (int64_t)(512 << 20) / (148 * tile_bytes));
         s.slab_tiles = std::min<int64_t>(s.tiles, 148 * waves);
         s.wtiles = (int)(ceil_div(2 * p.H, 128) * ceil_div(p.C, 128) + ceil_div(p.H, 128) * ceil_div(p.O, 128));
-        const int64_t pieces = s.slab_tiles * (TP / WForm<T>::KC);
+        const int64_t pieces = s.slab_tiles * (TP / (s.wide ? WForm<float>::KC : WForm<T>::KC));
         s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(148 / s.wtiles, pieces));
         s.z = at;
         at += up((size_t)s.slab_tiles * tile_bytes);
@@ -1796,7 +1835,8 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
     w.H = p.H;
     w.O = p.O;
     // x and e in place: whole tiles a sample, on 16-byte boundaries
-    const bool in_place = d.points % TP == 0 && aligned({o.x, g.gy}, 16);
+    const bool converted = z.wide && sizeof(T) == 2;
+    const bool in_place = !converted && d.points % TP == 0 && aligned({o.x, g.gy}, 16);
     w.rows = 3 * p.H + (in_place ? 0 : p.C + p.O);
     w.per_sample = in_place ? (int)(d.points / TP) : 0;
     q.z_rows = w.rows;
@@ -1813,25 +1853,40 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
             xs = const_cast<void*>(o.x);
             es = const_cast<void*>(g.gy);
         }
-        if (!row_map<T>(&mg, ws + z.z, TP, rows, imin(128, 2 * p.H)) || !row_map<T>(&mh, ws + z.z, TP, rows, imin(128, p.H)) ||
-            !row_map<T>(&mx, xs, in_place ? d.points : TP, in_place ? d.batch * p.C : rows, imin(128, p.C)) ||
-            !row_map<T>(&me, es, in_place ? d.points : TP, in_place ? d.batch * p.O : rows, imin(128, p.O)))
+        auto maps = [&](auto t) {
+            using Z = decltype(t);
+            return row_map<Z>(&mg, ws + z.z, TP, rows, imin(128, 2 * p.H)) &&
+                   row_map<Z>(&mh, ws + z.z, TP, rows, imin(128, p.H)) &&
+                   row_map<Z>(&mx, xs, in_place ? d.points : TP, in_place ? d.batch * p.C : rows, imin(128, p.C)) &&
+                   row_map<Z>(&me, es, in_place ? d.points : TP, in_place ? d.batch * p.O : rows, imin(128, p.O));
+        };
+        if (!(converted ? maps(float{}) : maps(T{})))
             return fail(NOP_E_CUDA, "cuTensorMapEncodeTiled failed");
     }
     const int64_t slab = weights ? z.slab_tiles : z.tiles;
-    constexpr int wsmem = WForm<T>::BODY + (int)sizeof(WBars);
     for (int64_t t = 0; t < z.tiles; t += slab) {
         q.tile0 = (int)t;
         q.tiles = (int)std::min<int64_t>(slab, z.tiles - t);
         const unsigned grid = (unsigned)std::min<int64_t>(q.tiles, dev.sms);
-        rc = d.activation == NOP_ACT_GELU ? launch<k_block<T, T, true, true>>(dev, grid, kThreads, p.smem, s, q, dev.status)
-                                          : launch<k_block<T, T, true, false>>(dev, grid, kThreads, p.smem, s, q, dev.status);
+        auto block = [&](auto wide) {
+            constexpr bool W = decltype(wide)::value;
+            return d.activation == NOP_ACT_GELU
+                       ? launch<k_block<T, T, true, true, W>>(dev, grid, kThreads, p.smem, s, q, dev.status)
+                       : launch<k_block<T, T, true, false, W>>(dev, grid, kThreads, p.smem, s, q, dev.status);
+        };
+        if constexpr (sizeof(T) == 2) rc = converted && weights ? block(std::true_type{}) : block(std::false_type{});
+        else rc = block(std::false_type{});
         if (rc != NOP_OK) return rc;
         if (!weights) continue;
-        w.pieces = q.tiles * (TP / WForm<T>::KC);
         w.tile0 = (int)t;
         w.accumulate = t > 0;
-        rc = launch<k_wgrad<T>>(dev, (unsigned)(z.splits * z.wtiles), WForm<T>::THREADS, wsmem, s, mg, mh, mx, me, w, dev.status);
+        auto contract = [&](auto t) {
+            using F = WForm<decltype(t)>;
+            w.pieces = q.tiles * (TP / F::KC);
+            return launch<k_wgrad<decltype(t)>>(dev, (unsigned)(z.splits * z.wtiles), F::THREADS,
+                                                F::BODY + (int)sizeof(WBars), s, mg, mh, mx, me, w, dev.status);
+        };
+        rc = converted ? contract(float{}) : contract(T{});
         if (rc != NOP_OK) return rc;
     }
     // dL/dx of the channels past the first launch's: the products again, without the scratch

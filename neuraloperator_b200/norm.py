@@ -12,6 +12,7 @@ residual's addition and an 8-bit output (nop_rms_norm_forward / nop_rms_norm_bac
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
@@ -48,6 +49,15 @@ def _desc(x: torch.Tensor, eps: float) -> _lib.NopNormDesc:
     for n in x.shape[2:]:
         points *= n
     return _lib.NopNormDesc(_lib.ABI_VERSION, _DTYPES[x.dtype], batch, points, channels, eps)
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(channels: int) -> int:
+    """Bytes of the backward's workspace: they depend on the channels alone."""
+    size = ctypes.c_size_t()
+    _lib.check(_lib.library().nop_rms_norm_backward_workspace_size(
+        _lib.NopNormDesc(_lib.ABI_VERSION, _lib.DTYPE_FP32, 1, 1, channels, 0.0), size))
+    return size.value
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
@@ -98,14 +108,11 @@ class _RMSNormFn(torch.autograd.Function):
         gx = torch.empty_like(r) if need_r else None
         need_w = need_w and weight is not None
         gw = torch.empty(r.shape[1], device=r.device, dtype=torch.float32) if need_w else None
-        desc, lib = _desc(r, ctx.eps), _lib.library()
-        ws, size = None, ctypes.c_size_t()
-        if need_w:
-            _lib.check(lib.nop_rms_norm_backward_workspace_size(desc, size))
-            ws = torch.empty(size.value, device=r.device, dtype=torch.uint8)
+        size = _workspace_bytes(r.shape[1]) if need_w else 0
+        ws = torch.empty(size, device=r.device, dtype=torch.uint8) if need_w else None
         w = _fp32(weight)
-        _lib.call(lib.nop_rms_norm_backward, r.device, desc, r.data_ptr(), _ptr(w), gy.data_ptr(), _ptr(gr), _ptr(gx),
-                  _ptr(gw), _ptr(ws), size.value)
+        _lib.call(_lib.library().nop_rms_norm_backward, r.device, _desc(r, ctx.eps), r.data_ptr(), _ptr(w), gy.data_ptr(),
+                  _ptr(gr), _ptr(gx), _ptr(gw), _ptr(ws), size)
         return (gx if need_x else None, gw.to(weight.dtype) if need_w else None, gx if need_res else None, None)
 
 
