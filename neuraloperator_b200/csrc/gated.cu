@@ -17,7 +17,7 @@
 // jobs' first products while the epilogue warps work on a job; a tile's D2 is read after the next tile's first middle.
 //
 // Operands.  16-bit fields multiply as they are (products exact, fp32 sums); h, dg and du go into their products in two
-// 16-bit parts (Mid), and into the weights' gradients rounded once.  fp32 values are split into three
+// 16-bit parts (Mid), and into the weights' gradients of many points rounded once.  fp32 values are split into three
 // bf16 parts, v = a + b + c to within 2^-26 |v|, and six of the nine products are summed (the three left out are
 // below 2^-26): fp32 accuracy at the cost of six 16-bit MMAs, the same tensor time as three tf32 passes on a
 // hi / lo split but three quarters of its shared memory, and 2^-26 instead of 2^-21.  The tensor core adds to its
