@@ -320,3 +320,12 @@ def test_offsets_past_32_bits():
         assert (gx[:, :, : p - n] == 0).all()
         assert _lib.device_status() == 0
         del x, y, gx
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_samples_of_whole_tiles(dtype):
+    """Samples of whole tiles, more points than the fp32 scratch of 16-bit fields takes: the fields are contracted in
+    place, over several samples; and the last size that takes that scratch, and the first that does not."""
+    check(operands(3, 48, 72, 40, (160, 128), dtype), "gelu")
+    check(operands(1, 20, 24, 20, (1 << 15,), dtype), "silu")
+    check(operands(1, 20, 24, 20, ((1 << 15) + 1,), dtype), "silu")
