@@ -434,7 +434,7 @@ int32_t nop_rms_norm_backward(const nop_norm_desc* desc, const void* r, const fl
  *   h = act(w_gate x + b_gate) * (w_up x + b_up),  y = w_down h + b_down      y [batch, out_channels, points]
  * w_gate, w_up [hidden, channels], w_down [out_channels, hidden], biases (each may be NULL) [hidden], [hidden],
  * [out_channels], all of the field's type `dtype`.  fp32 in fp32 accuracy; 16-bit types with fp32 sums and h to
- * twice the type's precision (rounded to the type in the weights' gradients of more than 2^15 points).  x_dtype: dtype, or NOP_DTYPE_E4M3 (forward only, 16-bit dtype) with x_scale [batch, points]
+ * twice the type's precision.  x_dtype: dtype, or NOP_DTYPE_E4M3 (forward only, 16-bit dtype) with x_scale [batch, points]
  * float32, the values being x * x_scale.  Values that are not finite, h among them (fp16: above 65504),
  * give results that are not finite at their point.  channels and out_channels <= 256, hidden <= 16384, fewer than 2^31 points. */
 typedef enum nop_activation { NOP_ACT_SILU = 0, NOP_ACT_GELU = 1 } nop_activation;

@@ -17,7 +17,7 @@
 // jobs' first products while the epilogue warps work on a job; a tile's D2 is read after the next tile's first middle.
 //
 // Operands.  16-bit fields multiply as they are (products exact, fp32 sums); h, dg and du go into their products in two
-// 16-bit parts (Mid), and into the weights' gradients of many points rounded once.  fp32 values are split into three
+// 16-bit parts (Mid), and into the weights' gradients in two bf16 parts or in fp32 (Scratch).  fp32 values are split into three
 // bf16 parts, v = a + b + c to within 2^-26 |v|, and six of the nine products are summed (the three left out are
 // below 2^-26): fp32 accuracy at the cost of six 16-bit MMAs, the same tensor time as three tf32 passes on a
 // hi / lo split but three quarters of its shared memory, and 2^-26 instead of 2^-21.  The tensor core adds to its
@@ -95,6 +95,18 @@ template <int SPL> struct Passes {
     __device__ static constexpr int b(int i) { return i == 1 || i == 3 ? 1 : i == 4 ? 2 : 0; }
 };
 
+// What the backward's scratch holds dg, du and h in: fp32 values of fp32 and fp16 fields (a gradient below 2^-24 or above
+// 65504 is not lost on its way into a sum), two bf16 parts of bf16 fields, which multiply as they lie.  Rounded once to
+// 16 bits they put the weights' gradients off by 1.4 times the result's own rounding.
+template <class T> struct Scratch {
+    using type = float;
+    static constexpr int PARTS = 1;
+};
+template <> struct Scratch<__nv_bfloat16> {
+    using type = __nv_bfloat16;
+    static constexpr int PARTS = 2;
+};
+
 // Warps of k_block.
 constexpr int kEpi = 8;                       // 0..7: middle and output
 constexpr int kProd = 4;                      // 8..11: x (and e) into shared memory
@@ -126,8 +138,8 @@ struct Params {
     const char* packed;
     const float* bias;         // the biases of g, u and (forward) of the output: fp32, padded with zeros
     void* out;                 // y, or dL/dx (may be NULL)
-    void* z;                   // backward: [tile][z_rows][128] dg, du, h (and x, e) (may be NULL)
-    int z_rows;                // 3 H, or 3 H + C + O
+    void* z;                   // backward: [tile][z_rows][128] dg, du, h (their second parts) (x, e) (may be NULL)
+    int z_rows;                // 3 H PARTS, or that and C + O
     uint32_t P, points;        // a sample's points, all points
     uint32_t p_mul, p_shift;   // n / P = n p_mul >> p_shift for n < 2^31
     int tile0, tiles;          // tiles of this launch
@@ -647,11 +659,11 @@ struct Bars {
     int abort_flag;
 };
 
-// WIDE: the scratch is fp32 (of a 16-bit field with few points)
-template <class T, class IN, bool BWD, bool GELU, bool WIDE = false>
+template <class T, class IN, bool BWD, bool GELU>
 __global__ void __launch_bounds__(kThreads, 1)
 k_block(const __grid_constant__ Params p, int* __restrict__ status) {
     constexpr int SPL = Form<T>::SPL, KC = Form<T>::KC, NP = Passes<SPL>::N, MID = Mid<T>::N;
+    constexpr bool WIDE = sizeof(typename Scratch<T>::type) > sizeof(T);  // an fp32 scratch of a 16-bit field
     extern __shared__ __align__(1024) char sm[];
     const Plan& pl = p.pl;
     Bars& bar = *reinterpret_cast<Bars*>(sm + pl.o_bar);
@@ -777,14 +789,15 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
             if (q.i == 0 && !wait(&bar.empty_a[slot], phase)) return false;  // (true of a new barrier's phase 1)
             char* s = sm + pl.o_a + slot * pl.a_slot;
             // x and e go to the scratch too, once a tile
-            const bool keep = BWD && p.z && p.z_rows > 3 * pl.H && q.j == 0;
+            const int results = 3 * Scratch<T>::PARTS * pl.H;
+            const bool keep = BWD && p.z && p.z_rows > results && q.j == 0;
             const int c0 = (is_x ? q.kc : q.kc - pl.nKx) * KC;
             auto one = [&](const Item<IN>& it, int i) {
                 const int ch = w + 4 * i;
                 if (ch * 8 < pw) store_item<T, IN>(it, s, ch, pw / 16, lane, p.vec);
                 if constexpr (BWD) {
                     const int64_t to =
-                        ((int64_t)(tile_at(q.k) - p.tile0) * p.z_rows + 3 * pl.H + (is_x ? 0 : pl.C)) * TP;
+                        ((int64_t)(tile_at(q.k) - p.tile0) * p.z_rows + results + (is_x ? 0 : pl.C)) * TP;
                     if (keep && WIDE)
                         copy_wide<T>(it, static_cast<float*>(p.z) + to, c0 + ch * 8, is_x ? pl.C : pl.O, lane);
                     else if (keep)
@@ -1116,11 +1129,15 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                             store_wide(zw + (pl.H + 2 * i) * TP, du, left - 2 * i);
                             store_wide(zw + (2 * pl.H + 2 * i) * TP, h, left - 2 * i);
                         } else if constexpr (SPL == 1) {
-                            uint32_t o[1];
-                            images<T>(h, o);
-                            store_rows(z + 2 * i * TP, t[0], lane, left - 2 * i);
-                            store_rows(zu + 2 * i * TP, r[0], lane, left - 2 * i);
-                            store_rows(zh + 2 * i * TP, o[0], lane, left - 2 * i);
+                            uint32_t o[MID];
+                            mid_images<T>(h, o);
+#pragma unroll
+                            for (int s = 0; s < MID; ++s) {
+                                const int at = (3 * s * pl.H + 2 * i) * TP;
+                                store_rows(z + at, t[s], lane, left - 2 * i);
+                                store_rows(zu + at, r[s], lane, left - 2 * i);
+                                store_rows(zh + at, o[s], lane, left - 2 * i);
+                            }
                         } else {
                             if (2 * i < left) {
                                 z[2 * i * TP] = dg.x;
@@ -1238,13 +1255,15 @@ constexpr int kPromote = 8;                   // pieces an accumulator runs befo
 constexpr int kImages = 2;                    // fp32: stages of split operands
 
 // A piece is 128 bytes of points of up to 128 rows of each operand, as a 128-byte-swizzled tensor copy leaves them:
-// for 16-bit types that is the MMA's own K-major layout and the pieces are multiplied as they land.
+// for bf16 that is the MMA's own K-major layout and the pieces are multiplied as they land, both parts of A with B.
 template <class T> struct WForm {
     // warps 0..7: accumulators; then fp32 splitting (four warps an operand) and row sums, MMA issue, copies
     static constexpr int WORK = sizeof(T) == 4 ? 8 : 4, MMA = 8 + WORK, LOAD = MMA + 1, THREADS = 32 * (LOAD + 1);
     static constexpr int KC = 128 / (int)sizeof(T);
-    static constexpr int STAGES = sizeof(T) == 4 ? 3 : 6;
-    static constexpr int RAW = 2 * 128 * 128;                        // A rows, then B rows
+    static constexpr int STAGES = sizeof(T) == 4 ? 3 : 4;
+    static constexpr int PARTS = Scratch<T>::PARTS;
+    static constexpr int ONE = 128 * 128;                            // bytes of one operand's rows
+    static constexpr int RAW = (1 + PARTS) * ONE;                    // A rows, then B rows, then A's second part
     static constexpr int IMG = sizeof(T) == 4 ? 128 * KC * 2 : 0;    // one image of one operand
     static constexpr int SPLIT = 2 * Form<T>::SPL * IMG;
     static constexpr int BODY = STAGES * RAW + (sizeof(T) == 4 ? kImages * SPLIT : 0);
@@ -1254,7 +1273,7 @@ struct WParams {
     float* partial;            // [split][tile][128][128]
     double* sums;              // [split][2 H + O] row sums of dg, du and e (may be NULL)
     int C, H, O;
-    int rows;                  // rows of a tile of the scratch
+    int rows;                  // rows of a tile of the scratch (3 H PARTS are dg, du and h)
     int tile0, per_sample;     // x and e in place: the slab's first tile, tiles of a sample; per_sample 0: in the scratch
     int pieces;                // pieces of KC points in the slab
     int splits;
@@ -1337,9 +1356,10 @@ k_wgrad(const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensor
         if (lane == 0) {
             const CUtensorMap* mb = of_x ? &mx : &me;
             const int a0 = (of_x ? 0 : 2 * p.H) + mt * 128;
-            const int b0 = nt * 128 + (p.per_sample ? 0 : 3 * p.H + (of_x ? 0 : p.C));
+            const int b0 = nt * 128 + (p.per_sample ? 0 : 3 * W::PARTS * p.H + (of_x ? 0 : p.C));
             const CUtensorMap* ma = of_x ? &mg : &mh;
-            const uint32_t bytes = (uint32_t)(imin(128, of_x ? 2 * p.H : p.H) + imin(128, of_x ? p.C : p.O)) * 128;
+            const uint32_t bytes =
+                (uint32_t)(W::PARTS * imin(128, of_x ? 2 * p.H : p.H) + imin(128, of_x ? p.C : p.O)) * 128;
             int k = 0;
             for (; k < steps; ++k) {
                 const int slot = k % S, use = k / S;
@@ -1357,11 +1377,12 @@ k_wgrad(const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensor
                         : "memory");
                 };
                 copy(dst, ma, c, t * p.rows + a0);
+                if (W::PARTS > 1) copy(dst + 2 * W::ONE, ma, c, t * p.rows + 3 * p.H + a0);
                 if (p.per_sample) {
                     const int s = (p.tile0 + t) / p.per_sample, first = (p.tile0 + t - s * p.per_sample) * TP;
-                    copy(dst + W::RAW / 2, mb, first + c, s * (of_x ? p.C : p.O) + b0);
+                    copy(dst + W::ONE, mb, first + c, s * (of_x ? p.C : p.O) + b0);
                 } else {
-                    copy(dst + W::RAW / 2, mb, c, t * p.rows + b0);
+                    copy(dst + W::ONE, mb, c, t * p.rows + b0);
                 }
             }
             for (int i = 0; i < S && i < k; ++i)  // no copy outlives the CTA (bounded)
@@ -1397,7 +1418,7 @@ k_wgrad(const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensor
                 const int si = k % kImages, use = k / kImages;
                 if (use > 0 && !wait(&bar.img_free[si], (uint32_t)(use - 1) & 1)) break;
                 if (!o || r < n) {
-                    row_of(raw + o * (W::RAW / 2), v);
+                    row_of(raw + o * W::ONE, v);
                     char* to = split_at + si * W::SPLIT + o * SPL * W::IMG + (r >> 3) * 256 + (r & 7) * 16;
 #pragma unroll
                     for (int ch = 0; ch < KC / 8; ++ch) {
@@ -1412,8 +1433,12 @@ k_wgrad(const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensor
                     if (summing) add(v);
                 }
             } else {
-                row_of(raw + o * (W::RAW / 2), v);
+                row_of(raw + o * W::ONE, v);
                 add(v);
+                if (W::PARTS > 1 && !o) {
+                    row_of(raw + 2 * W::ONE, v);
+                    add(v);
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -1462,9 +1487,12 @@ k_wgrad(const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensor
                     commit(&bar.img_free[slot], leader);
                 } else {
                     const uint32_t at = tc::smem_u32(sm + slot * W::RAW);
-                    const uint64_t a0 = desc_128b(at), b0 = desc_128b(at + W::RAW / 2);
+                    const uint64_t a0 = desc_128b(at), b0 = desc_128b(at + W::ONE), a1 = desc_128b(at + 2 * W::ONE);
 #pragma unroll
-                    for (int ks = 0; ks < KC / 16; ++ks) mma_ss(d, a0 + 2 * ks, b0 + 2 * ks, id, ks > 0 || !first, leader);
+                    for (int ks = 0; ks < KC / 16; ++ks) {
+                        mma_ss(d, a0 + 2 * ks, b0 + 2 * ks, id, ks > 0 || !first, leader);
+                        mma_ss(d, a1 + 2 * ks, b0 + 2 * ks, id, true, leader);
+                    }
                     commit(&bar.raw_free[slot], leader);
                 }
                 if (++slot == Q) {
@@ -1647,13 +1675,7 @@ struct Sizes {
     size_t packed, vec, z, partial, sums, bytes;
     int64_t slab_tiles, tiles;
     int splits, wtiles;
-    bool wide;
 };
-
-// A 16-bit field's dg, du and h are rounded for the weights' gradients, by as much as the gradients are.  Over many
-// points that averages (1.4 times the result's own rounding); with few, an element could be off by twice it, and the
-// scratch is fp32, at a cost that is small there: the fp32 path of k_wgrad.
-constexpr int64_t kWidePoints = 1 << 15;
 
 template <class T>
 Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd) {
@@ -1674,12 +1696,12 @@ Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd) {
         // The scratch of a slab: up to 512 MB, in whole waves of 148 tiles.  Slabs that stay in L2 save the scratch's
         // trip through HBM but lose more to their launches' beginnings and ends: 64 MB slabs took 2207 us where
         // 512 MB take 1646 (fp32, 64 channels, hidden 128, 2^20 points), and larger ones 1626.
-        s.wide = sizeof(T) == 4 || s.tiles * TP <= kWidePoints;
-        const int64_t tile_bytes = (int64_t)(3 * p.H + p.C + p.O) * TP * (s.wide ? 4 : 2);
+        using Z = typename Scratch<T>::type;
+        const int64_t tile_bytes = (int64_t)(3 * Scratch<T>::PARTS * p.H + p.C + p.O) * TP * sizeof(Z);
         const int64_t waves = std::max<int64_t>(1, (int64_t)(512 << 20) / (148 * tile_bytes));
         s.slab_tiles = std::min<int64_t>(s.tiles, 148 * waves);
         s.wtiles = (int)(ceil_div(2 * p.H, 128) * ceil_div(p.C, 128) + ceil_div(p.H, 128) * ceil_div(p.O, 128));
-        const int64_t pieces = s.slab_tiles * (TP / (s.wide ? WForm<float>::KC : WForm<T>::KC));
+        const int64_t pieces = s.slab_tiles * (TP / WForm<Z>::KC);
         s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(148 / s.wtiles, pieces));
         s.z = at;
         at += up((size_t)s.slab_tiles * tile_bytes);
@@ -1834,10 +1856,10 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
     w.C = p.C;
     w.H = p.H;
     w.O = p.O;
-    // x and e in place: whole tiles a sample, on 16-byte boundaries
-    const bool converted = z.wide && sizeof(T) == 2;
-    const bool in_place = !converted && d.points % TP == 0 && aligned({o.x, g.gy}, 16);
-    w.rows = 3 * p.H + (in_place ? 0 : p.C + p.O);
+    using Z = typename Scratch<T>::type;
+    // x and e in place: of the scratch's type, whole tiles a sample, on 16-byte boundaries
+    const bool in_place = std::is_same<Z, T>::value && d.points % TP == 0 && aligned({o.x, g.gy}, 16);
+    w.rows = 3 * Scratch<T>::PARTS * p.H + (in_place ? 0 : p.C + p.O);
     w.per_sample = in_place ? (int)(d.points / TP) : 0;
     q.z_rows = w.rows;
     w.nC = (int)ceil_div(p.C, 128);
@@ -1853,14 +1875,10 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
             xs = const_cast<void*>(o.x);
             es = const_cast<void*>(g.gy);
         }
-        auto maps = [&](auto t) {
-            using Z = decltype(t);
-            return row_map<Z>(&mg, ws + z.z, TP, rows, imin(128, 2 * p.H)) &&
-                   row_map<Z>(&mh, ws + z.z, TP, rows, imin(128, p.H)) &&
-                   row_map<Z>(&mx, xs, in_place ? d.points : TP, in_place ? d.batch * p.C : rows, imin(128, p.C)) &&
-                   row_map<Z>(&me, es, in_place ? d.points : TP, in_place ? d.batch * p.O : rows, imin(128, p.O));
-        };
-        if (!(converted ? maps(float{}) : maps(T{})))
+        if (!(row_map<Z>(&mg, ws + z.z, TP, rows, imin(128, 2 * p.H)) &&
+              row_map<Z>(&mh, ws + z.z, TP, rows, imin(128, p.H)) &&
+              row_map<Z>(&mx, xs, in_place ? d.points : TP, in_place ? d.batch * p.C : rows, imin(128, p.C)) &&
+              row_map<Z>(&me, es, in_place ? d.points : TP, in_place ? d.batch * p.O : rows, imin(128, p.O))))
             return fail(NOP_E_CUDA, "cuTensorMapEncodeTiled failed");
     }
     const int64_t slab = weights ? z.slab_tiles : z.tiles;
@@ -1868,25 +1886,16 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
         q.tile0 = (int)t;
         q.tiles = (int)std::min<int64_t>(slab, z.tiles - t);
         const unsigned grid = (unsigned)std::min<int64_t>(q.tiles, dev.sms);
-        auto block = [&](auto wide) {
-            constexpr bool W = decltype(wide)::value;
-            return d.activation == NOP_ACT_GELU
-                       ? launch<k_block<T, T, true, true, W>>(dev, grid, kThreads, p.smem, s, q, dev.status)
-                       : launch<k_block<T, T, true, false, W>>(dev, grid, kThreads, p.smem, s, q, dev.status);
-        };
-        if constexpr (sizeof(T) == 2) rc = converted && weights ? block(std::true_type{}) : block(std::false_type{});
-        else rc = block(std::false_type{});
+        rc = d.activation == NOP_ACT_GELU ? launch<k_block<T, T, true, true>>(dev, grid, kThreads, p.smem, s, q, dev.status)
+                                          : launch<k_block<T, T, true, false>>(dev, grid, kThreads, p.smem, s, q, dev.status);
         if (rc != NOP_OK) return rc;
         if (!weights) continue;
         w.tile0 = (int)t;
         w.accumulate = t > 0;
-        auto contract = [&](auto t) {
-            using F = WForm<decltype(t)>;
-            w.pieces = q.tiles * (TP / F::KC);
-            return launch<k_wgrad<decltype(t)>>(dev, (unsigned)(z.splits * z.wtiles), F::THREADS,
-                                                F::BODY + (int)sizeof(WBars), s, mg, mh, mx, me, w, dev.status);
-        };
-        rc = converted ? contract(float{}) : contract(T{});
+        using F = WForm<Z>;
+        w.pieces = q.tiles * (TP / F::KC);
+        rc = launch<k_wgrad<Z>>(dev, (unsigned)(z.splits * z.wtiles), F::THREADS, F::BODY + (int)sizeof(WBars), s, mg, mh, mx,
+                                me, w, dev.status);
         if (rc != NOP_OK) return rc;
     }
     // dL/dx of the channels past the first launch's: the products again, without the scratch
