@@ -13,8 +13,9 @@
 //   middle          the epilogue warps read D1, apply the activation and write h (backward: dg, du) back into the
 //                   same columns of tensor memory as the next A operand -- h never leaves the SM in the forward
 //   second product  D2 += h W_down^T (backward: dg W_gate + du W_up), A from tensor memory
-// and after a tile's last chunk D2 goes out.  Two or three D1 buffers take turns, so the tensor core works on the next
-// jobs' first products while the epilogue warps work on a job; a tile's D2 is read after the next tile's first middle.
+// and after a tile's last chunk (fp32: after every kRunSteps steps) D2 goes out.  Two or three D1 buffers take turns, so the
+// tensor core works on the next jobs' first products while the epilogue warps work on a job; a tile's D2 is read after the
+// next tile's first middle.
 //
 // Operands.  16-bit fields multiply as they are (products exact, fp32 sums); h, dg and du go into their products in two
 // 16-bit parts (Mid), and into the weights' gradients in two bf16 parts or in fp32 (Scratch).  fp32 values are split into three
@@ -114,6 +115,11 @@ constexpr int kMma = kEpi + kProd;            // 12: MMA issue
 constexpr int kLoad = kMma + 1;               // 13: weight copies
 constexpr int kThreads = 32 * (kLoad + 1);    // 14 warps: 128 registers a thread
 
+// fp32: K steps (of 16 hidden channels) that D2 runs before it is added to the output.  Every step truncates D2 by about
+// 2^-25 of it, always towards zero, so a sum over a whole wide hidden layer drifts: 1.7e-5 in y and 3.8e-5 in dL/dx at a
+// width of 16384, where 32 steps are below 1e-6.  16-bit results are rounded by far more.
+constexpr int kRunSteps = 32;
+
 struct Plan {
     int C, H, O;               // channels of x, hidden width, channels of y
     int Kx, Ky;                // padded K of the first products (Ky: backward only, 0 otherwise)
@@ -121,6 +127,7 @@ struct Plan {
     int N2;                    // padded columns of D2
     int n_d1, n_d2;            // D1 buffers (jobs in flight), D2 buffers
     int NH, nJ;                // chunk width, chunks
+    int per, runs;             // chunks that D2 runs before it goes out, times it goes out a tile
     int nKx, nKy, nH;          // ring pieces: of x, of e, of a chunk in the second product
     int na, nb;                // ring slots (nb: streaming)
     int reuse;                 // 1: a tile's A pieces stay in the ring for all its chunks
@@ -725,9 +732,9 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
     const int d2w = pl.N2 * (SPL == 3 ? 2 : 1);           // columns of a D2 buffer (D2c after D2)
     const uint32_t d2_0 = tmem + pl.n_d1 * d1w;
     const int lead = pl.n_d1 - 1;                         // first products run so many jobs ahead of second ones
-    // D2 buffer of this CTA's tile k, and how often it was used before
-    auto d2_buf = [&](int k) { return pl.n_d2 == 2 ? k & 1 : 0; };
-    auto d2_use = [&](int k) { return pl.n_d2 == 2 ? k >> 1 : k; };
+    // D2 buffer of this CTA's run q, and how often it was used before
+    auto d2_buf = [&](int q) { return pl.n_d2 == 2 ? q & 1 : 0; };
+    auto d2_use = [&](int q) { return pl.n_d2 == 2 ? q >> 1 : q; };
     auto tile_at = [&](int k) { return (uint32_t)(p.tile0 + (int)blockIdx.x + k * (int)gridDim.x); };
 
     if (warp >= kEpi && warp < kMma) {
@@ -959,7 +966,8 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                     }
                 }
             };
-            int j1 = 0, j2 = 0, k2 = 0;    // chunk of the first and of the second product, tile of the second
+            int j1 = 0, j2 = 0;            // chunk of the first and of the second product
+            int i2 = 0, q2 = 0;            // the second one's chunk of its run of D2, and the run
             int b1 = 0, b2 = 0;            // D1 buffers of the two
             uint32_t p1 = 1, p2 = 0;       // phases: of the first one's last second product, of the second one's middle
             for (int J = 0; J < jobs + lead && ok; ++J) {
@@ -1002,8 +1010,8 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                 }
                 if (J >= lead) {  // second product of job J - lead
                     if (!all(&bar.mid[b2], p2)) break;
-                    const int e = d2_buf(k2);
-                    if (j2 == 0 && d2_use(k2) > 0 && !all(&bar.d2_free[e], (uint32_t)(d2_use(k2) - 1) & 1)) break;
+                    const int e = d2_buf(q2);
+                    if (i2 == 0 && d2_use(q2) > 0 && !all(&bar.d2_free[e], (uint32_t)(d2_use(q2) - 1) & 1)) break;
                     const uint32_t d2 = d2_0 + e * d2w;
                     fence_after();
                     const uint32_t d = tmem + b2 * d1w;
@@ -1024,7 +1032,7 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                             const uint32_t wb = weights(at);
                             if (!ok) break;
                             fence_after();
-                            product_ts(d2, col, wb, pl.N2, pw, j2 != 0 || m != 0 || kc != 0, kc * (KC / 16));
+                            product_ts(d2, col, wb, pl.N2, pw, i2 != 0 || m != 0 || kc != 0, kc * (KC / 16));
                             at += pl.N2 * pw * 2 * SPL;
                             weights_done();
                         }
@@ -1035,10 +1043,11 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                         b2 = 0;
                         p2 ^= 1;
                     }
-                    if (++j2 == pl.nJ) {
+                    if (++j2 == pl.nJ) j2 = 0;
+                    if (++i2 == pl.per || j2 == 0) {
                         commit(&bar.d2[e], leader);
-                        j2 = 0;
-                        ++k2;
+                        i2 = 0;
+                        ++q2;
                     }
                 }
             }
@@ -1176,14 +1185,15 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
             }
             return true;
         };
-        auto output = [&](int k) -> bool {
+        // run r of tile k, the CTA's run q
+        auto output = [&](int k, int r, int q) -> bool {
             const uint32_t n = tile_at(k) * TP + row;
             const bool valid = n < p.points;
             const int width = BWD ? pl.C : pl.O;      // the field's channels
             const uint32_t b = valid ? sample_of(p, n) : 0;
             T* y = static_cast<T*>(p.out) + ((int64_t)b * width + pl.col0) * p.P + (valid ? n - b * p.P : 0);
-            const int e = d2_buf(k);
-            if (!wait(&bar.d2[e], (uint32_t)d2_use(k) & 1)) return false;
+            const int e = d2_buf(q);
+            if (!wait(&bar.d2[e], (uint32_t)d2_use(q) & 1)) return false;
             fence_after();
             const uint32_t d2 = d2_0 + e * d2w;
             const int n16 = pl.N2 / 16;
@@ -1208,7 +1218,7 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&bar.d2_free[e]);
                 }
-                if constexpr (!BWD) {  // all loads before the stores, which might alias them for all the compiler knows
+                if (!BWD && r == pl.runs - 1) {  // all loads before the stores, which might alias them for all the compiler knows
                     const float4* b2 = reinterpret_cast<const float4*>(bias_2 + 16 * g);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -1222,6 +1232,13 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
                 if (!valid || !p.out) continue;
                 T* yg = y + (int64_t)(16 * g) * p.P;
                 const int left = pl.cols - 16 * g;
+                if constexpr (SPL == 3) {
+                    if (r > 0) {  // the runs before this one, which this thread has written
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (i < left) v[i] += to_f(yg[(int64_t)i * p.P]);
+                    }
+                }
                 if (left >= 16) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) yg[(int64_t)i * p.P] = from_f<T>(v[i]);
@@ -1233,14 +1250,25 @@ k_block(const __grid_constant__ Params p, int* __restrict__ status) {
             }
             return true;
         };
+        // a run goes out after the next one's first middle
         bool ok = true;
+        int q = 0, k0 = 0, r0 = 0;  // runs begun; tile and place in it of the last one
         for (int k = 0; k < my && ok; ++k) {
-            for (int j = 0; j < pl.nJ && ok; ++j) {
+            for (int j = 0, i = 0, r = 0; j < pl.nJ && ok; ++j) {
                 ok = middle(k, j);
-                if (ok && j == 0 && k > 0) ok = output(k - 1);
+                if (i == 0) {
+                    if (ok && q > 0) ok = output(k0, r0, q - 1);
+                    ++q;
+                    k0 = k;
+                    r0 = r;
+                }
+                if (++i == pl.per) {
+                    i = 0;
+                    ++r;
+                }
             }
         }
-        if (ok && my > 0) output(my - 1);
+        if (ok && my > 0) output(k0, r0, q - 1);
     }
     fence_before();
     __syncthreads();
@@ -1627,6 +1655,8 @@ bool make_plan(const nop_gated_desc& d, bool bwd, int col0, Plan* out) {
     const int most = bwd && p.N2 * (SPL == 3 ? 2 : 1) > 128 ? 32 : 64;
     p.nJ = (p.H + most - 1) / most;
     p.NH = up16((p.H + p.nJ - 1) / p.nJ);
+    p.per = SPL == 3 ? imin(p.nJ, std::max(1, kRunSteps / (p.NH / 16 * (bwd ? 2 : 1)))) : p.nJ;
+    p.runs = (p.nJ + p.per - 1) / p.per;
     const int w1 = (bwd ? 3 : 2) * p.NH, w2 = p.N2 * (SPL == 3 ? 2 : 1);
     p.n_d1 = 3 * w1 + w2 <= 512 ? 3 : 2;
     p.n_d2 = p.n_d1 * w1 + 2 * w2 <= 512 ? 2 : 1;

@@ -120,3 +120,23 @@ def test_the_bound_notices_one_rounding(dtype):
             a, b = got[k].detach(), want[k].detach()
             err = float((a.to(dtype).double() - b).norm())
             assert (err <= allowed(b, sizes[k].detach(), dtype)) == inside, k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("h", [300, 513, 4096, 16384])
+@pytest.mark.parametrize("c, o", [(32, 32), (20, 150), (150, 20)])
+def test_wide_hidden_layers(h, c, o):
+    """fp32 sums over the hidden layer do not drift with its width.  Every add to a tensor-core accumulator truncates it by
+    at most 2^-25: 6 C / 16 adds of the first product in each of g, u and f, 32 of a part of the second one, and one fp32
+    rounding for each part that joins them."""
+    ops = operands(1, c, h, o, (300,), torch.float32, seed=11)
+    leaves = [t.clone().requires_grad_() for t in ops]
+    y = nb.gated_mlp(*leaves)
+    gy = make(y.shape, torch.float32, 12)
+    got = [y, *torch.autograd.grad(y, leaves, gy)]
+    adds = 3 * 6 * max(c, o) / 16 + 32 + 2 * h / 256
+    for name, a, b, size in zip(("y", "x"), got, *define_detached(ops, gy, "silu")):
+        scale = min(float(size.norm()), 2 * float(b.norm()))
+        # the activation's own error (1.5e-7 and its special functions, 2^-22) on the way
+        assert float((a.detach().double() - b).norm()) <= scale * (adds * 2.0 ** -25 + 6e-7), name
+    check(ops, "gelu")
