@@ -326,7 +326,8 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // other one
 __device__ __forceinline__ float2 rcp2(float2 v) { return __fmul2_rn(both(rcp_approx(v.x * v.y)), make_float2(v.y, v.x)); }
 
-// act(g) and act'(g) of two values.  SiLU: g s, s (1 + g (1 - s)), s = 1 / (1 + exp(-g)).  GELU: g P(g),
+// act(g) and act'(g) of two values.  SiLU: g s, s + g s (1 - s), s = 1 / (1 + exp(-g)), where 1 - s = exp(-g) s: a
+// subtraction would leave the reciprocal's last bit, which g multiplies (slope 1e-3 off at g = 1e4).  GELU: g P(g),
 // P(g) + g p(g) with the normal distribution function P from erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2),
 // t = 1 / (1 + q x), Abramowitz & Stegun, Handbook of Mathematical Functions (1964), eq. 7.1.26 (|error| <= 1.5e-7);
 // its exponential is also the density's.  Reciprocal and exponential are the special-function unit's (2^-22 or so).
@@ -335,10 +336,10 @@ __device__ __forceinline__ float2 activation(float2 g, float2& slope) {
     if (!GELU) {
         // below g = -41 the exponential is held at 2^60 (the product of two stays finite): |silu| < 1e-16 |g| there
         const float2 t = __fmul2_rn(g, both(-1.4426950408889634f));
-        const float2 d = __fadd2_rn(make_float2(exp2_approx(fminf(t.x, 60.f)), exp2_approx(fminf(t.y, 60.f))), both(1.f));
-        const float2 s = rcp2(d);
+        const float2 e = make_float2(exp2_approx(fminf(t.x, 60.f)), exp2_approx(fminf(t.y, 60.f)));
+        const float2 s = rcp2(__fadd2_rn(e, both(1.f)));
         const float2 a = __fmul2_rn(g, s);
-        slope = __ffma2_rn(a, __ffma2_rn(s, both(-1.f), both(1.f)), s);
+        slope = __ffma2_rn(a, __fmul2_rn(e, s), s);
         return a;
     }
     const float2 x = make_float2(fabsf(g.x), fabsf(g.y));  // |g| = sqrt(2) times erfc's argument

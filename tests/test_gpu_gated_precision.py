@@ -140,3 +140,35 @@ def test_wide_hidden_layers(h, c, o):
         # the activation's own error (1.5e-7 and its special functions, 2^-22) on the way
         assert float((a.detach().double() - b).norm()) <= scale * (adds * 2.0 ** -25 + 6e-7), name
     check(ops, "gelu")
+
+
+def values_and_slopes(gates, act):
+    """act(g) and act'(g) of every gate, each in a hidden channel of its own: x = 1, up = 1, the outputs one hidden channel
+    each (256 a call), and the gradient of the gate's bias."""
+    acts, slopes = [], []
+    for part in gates.split(256):
+        h = part.numel()
+        bias = torch.zeros(h, device="cuda", requires_grad=True)
+        ones = torch.ones(h, 1, device="cuda")
+        y = nb.gated_mlp(torch.ones(1, 1, 1, device="cuda"), part[:, None], ones, torch.eye(h, device="cuda"), bias,
+                         activation=act)
+        slopes.append(torch.autograd.grad(y, bias, torch.ones_like(y))[0])
+        acts.append(y.detach()[0, :, 0])
+    return torch.cat(acts).double(), torch.cat(slopes).double()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("gate", [None, 50.0, 200.0, 1e3, 1e4, -50.0, -1e4])
+def test_slope_of_every_gate(gate, act):
+    """Elementwise; hidden channels go through the activation in pairs, so a saturated gate stands beside a small one."""
+    g = (torch.rand(4096, generator=torch.Generator("cuda").manual_seed(2), device="cuda") - 0.5) * 24
+    if gate is not None:
+        g[0::2] = gate
+    ref = g.double().requires_grad_()
+    want = (F.silu if act == "silu" else F.gelu)(ref)
+    (slope,) = torch.autograd.grad(want.sum(), ref)
+    a, s = values_and_slopes(g, act)
+    # exponential and reciprocal: some 2^-22 of a slope of at most 1.13; the normal distribution's approximation: 1.5e-7
+    assert float((s - slope).abs().max()) <= 1.5e-6
+    assert float(((a - want.detach()).abs() / (1 + g.abs())).max()) <= 1.5e-6
