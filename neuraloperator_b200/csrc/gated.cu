@@ -321,6 +321,11 @@ __device__ __forceinline__ float rcp_approx(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // two reciprocals for one special-function operation, which bound the middle (16 a cycle and SM): 1 / (x y) times the
 // other one
@@ -334,11 +339,12 @@ __device__ __forceinline__ float2 rcp2(float2 v) { return __fmul2_rn(both(rcp_ap
 template <bool GELU>
 __device__ __forceinline__ float2 activation(float2 g, float2& slope) {
     if (!GELU) {
-        // below g = -41 the exponential is held at 2^60 (the product of two stays finite): |silu| < 1e-16 |g| there
-        const float2 t = __fmul2_rn(g, both(-1.4426950408889634f));
-        const float2 e = make_float2(exp2_approx(fminf(t.x, 60.f)), exp2_approx(fminf(t.y, 60.f)));
+        // g is held at -60 ln 2, where |silu| < 4e-17: the exponential is 2^60 there, and the product of two is finite
+        const float2 c = make_float2(max_nan(g.x, -41.588830834f), max_nan(g.y, -41.588830834f));
+        const float2 t = __fmul2_rn(c, both(-1.4426950408889634f));
+        const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
         const float2 s = rcp2(__fadd2_rn(e, both(1.f)));
-        const float2 a = __fmul2_rn(g, s);
+        const float2 a = __fmul2_rn(c, s);
         slope = __ffma2_rn(a, __fmul2_rn(e, s), s);
         return a;
     }

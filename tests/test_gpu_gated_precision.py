@@ -172,3 +172,27 @@ def test_slope_of_every_gate(gate, act):
     # exponential and reciprocal: some 2^-22 of a slope of at most 1.13; the normal distribution's approximation: 1.5e-7
     assert float((s - slope).abs().max()) <= 1.5e-6
     assert float(((a - want.detach()).abs() / (1 + g.abs())).max()) <= 1.5e-6
+
+
+def check_huge(gate, act):
+    """Hidden channels of a huge gate and of small ones in turn, each with an output of its own."""
+    g = (torch.rand(256, generator=torch.Generator("cuda").manual_seed(3), device="cuda") - 0.5) * 12
+    g[0::2] = gate
+    ref = g.double().requires_grad_()
+    want = (F.silu if act == "silu" else F.gelu)(ref)
+    (slope,) = torch.autograd.grad(want.sum(), ref)
+    a, s = values_and_slopes(g, act)
+    assert float((a[1::2] - want[1::2].detach()).abs().max()) <= 1.5e-6 * 7
+    assert float((s - slope).abs().max()) <= 1.5e-6
+    if gate > 0:
+        assert float((a[0::2] / gate - 1).abs().max()) <= 1e-6
+    else:
+        assert float(a[0::2].abs().max()) <= 1e-15
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", [-1e4, -1e20, torch.finfo(torch.float32).min / 2])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_far_below_zero_are_shut(gate, act):
+    """However far below zero, as a bias that switches hidden channels off would have it."""
+    check_huge(gate, act)
