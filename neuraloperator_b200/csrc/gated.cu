@@ -348,7 +348,9 @@ __device__ __forceinline__ float2 activation(float2 g, float2& slope) {
         slope = __ffma2_rn(a, __fmul2_rn(e, s), s);
         return a;
     }
-    const float2 x = make_float2(fabsf(g.x), fabsf(g.y));  // |g| = sqrt(2) times erfc's argument
+    // |g| = sqrt(2) times erfc's argument; the exponential is zero long before 64, and the product of two denominators
+    // has to be finite (a neighbour of a gate of 3e38 came out as if it were saturated)
+    const float2 x = make_float2(fminf(fabsf(g.x), 64.f), fminf(fabsf(g.y), 64.f));
     const float2 d = __ffma2_rn(x, both(0.3275911f * 0.70710678118654752f), both(1.f));
     const float2 t = rcp2(d);
     const float2 q = __fmul2_rn(__fmul2_rn(g, g), both(-0.5f * 1.4426950408889634f));

@@ -196,3 +196,11 @@ def check_huge(gate, act):
 def test_gates_far_below_zero_are_shut(gate, act):
     """However far below zero, as a bias that switches hidden channels off would have it."""
     check_huge(gate, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", [1e20, 3e38, -3e38])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_huge_gates_leave_their_neighbours(gate, act):
+    """Gates whose products overflow fp32 share a reciprocal with small ones."""
+    check_huge(gate, act)
