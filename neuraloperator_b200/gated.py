@@ -16,6 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .utils import dense
 
 _DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
@@ -82,10 +83,6 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or (t.is_contiguous() and not t.requires_grad) else t.detach().contiguous()
-
-
 def _workspace(lib, desc, backward: int, device) -> torch.Tensor:
     size = ctypes.c_size_t()
     _lib.check(lib.nop_gated_workspace_size(desc, backward, size))
@@ -93,7 +90,7 @@ def _workspace(lib, desc, backward: int, device) -> torch.Tensor:
 
 
 def _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, x_scale, hidden, out):
-    tensors = [_dense(t) for t in (x, x_scale, w_gate, w_up, w_down, b_gate, b_up, b_down)]
+    tensors = [dense(t) for t in (x, x_scale, w_gate, w_up, w_down, b_gate, b_up, b_down)]
     y = torch.empty((x.shape[0], out, *x.shape[2:]), device=x.device, dtype=w_gate.dtype)
     lib, desc = _lib.library(), _desc(x, w_gate.dtype, hidden, out, activation)
     ws = _workspace(lib, desc, 0, x.device)
@@ -114,8 +111,8 @@ class _GatedFn(torch.autograd.Function):
     def backward(ctx, gy):
         activation, hidden, out = ctx.cfg
         saved = ctx.saved_tensors
-        x, w_gate, w_up, w_down, b_gate, b_up, b_down = [_dense(t) for t in saved]
-        gy = gy.contiguous()
+        x, w_gate, w_up, w_down, b_gate, b_up, b_down = [dense(t) for t in saved]
+        gy = dense(gy)
         grads = [torch.empty(t.shape, device=x.device, dtype=t.dtype) if t is not None and need else None
                  for t, need in zip(saved, ctx.needs_input_grad)]
         lib, desc = _lib.library(), _desc(x, w_gate.dtype, hidden, out, activation)

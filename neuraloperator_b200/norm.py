@@ -20,6 +20,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .utils import dense
 
 _DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
@@ -60,14 +61,10 @@ def _workspace_bytes(channels: int) -> int:
     return size.value
 
 
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    return t if t.is_contiguous() and not t.requires_grad else t.detach().contiguous()
-
-
 def _fp32(weight: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    if weight is None or (weight.dtype is torch.float32 and weight.is_contiguous()):
+    if weight is None or (weight.dtype is torch.float32 and weight.is_contiguous() and not weight.is_neg()):
         return weight
-    return weight.detach().to(torch.float32).contiguous()
+    return dense(weight.detach().to(torch.float32))
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -76,8 +73,7 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _forward(x, weight, residual, eps):
     """(y, r): r is x itself without a residual."""
-    x = _dense(x)
-    residual = None if residual is None else _dense(residual)
+    x, residual = dense(x), dense(residual)
     y = torch.empty_like(x)
     r = x if residual is None else torch.empty_like(x)
     w = _fp32(weight)
@@ -103,8 +99,8 @@ class _RMSNormFn(torch.autograd.Function):
         if gy is None:  # only the sum was used
             return gr if need_x else None, None, gr if need_res else None, None
         need_r = need_x or need_res
-        gy = gy.contiguous()
-        gr = gr.contiguous() if gr is not None and need_r else None
+        gy = dense(gy)
+        gr = dense(gr) if need_r else None
         gx = torch.empty_like(r) if need_r else None
         need_w = need_w and weight is not None
         gw = torch.empty(r.shape[1], device=r.device, dtype=torch.float32) if need_w else None
@@ -137,8 +133,7 @@ def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_quantized has no backward; call it under torch.no_grad()")
-    x = _dense(x)
-    residual = None if residual is None else _dense(residual)
+    x, residual = dense(x), dense(residual)
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty((x.shape[0], 1, *x.shape[2:]), device=x.device, dtype=torch.float32)
     r = None if residual is None else torch.empty_like(x)

@@ -38,6 +38,16 @@ def grad_needed(x: torch.Tensor, module: torch.nn.Module) -> bool:
     return x.requires_grad or any(p.requires_grad for p in module.parameters())
 
 
+def dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t's values in contiguous memory, apart from autograd, for a kernel that reads its pointer: a lazily negated tensor
+    is contiguous too, and its memory holds the values with the other sign."""
+    if t is None:
+        return None
+    if t.is_neg():
+        return t.detach().resolve_neg().contiguous()
+    return t if t.is_contiguous() and not t.requires_grad else t.detach().contiguous()
+
+
 def count_model_params(model) -> int:
     """Parameter count with complex entries counted twice (neuralop/utils.py:19-28)."""
     return sum(p.numel() * 2 if p.is_complex() else p.numel() for p in model.parameters())

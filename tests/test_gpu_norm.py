@@ -251,3 +251,29 @@ def test_offsets_past_32_bits():
     xs = x.detach()[..., tail].clone().requires_grad_()
     (want,) = torch.autograd.grad(nb.rms_norm(xs, w, eps=EPS), xs, g[..., tail].contiguous())
     assert torch.equal(gx[..., tail], want)
+
+
+def negated(t):
+    """The same values as t, held with the other sign and a mark (as z.conj().imag is)."""
+    n = torch._neg_view(-t)
+    assert n.is_neg() and n.is_contiguous() and torch.equal(n, t)
+    return n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lazily_negated_tensors(dtype):
+    x, res, w = make((2, 12, 30), dtype, 1), make((2, 12, 30), dtype, 2), make((12,), torch.float32, 3)
+    gy, gr = make(x.shape, dtype, 4), make(x.shape, dtype, 5)
+    with torch.no_grad():
+        for a, b in zip(nb.rms_norm(negated(x), negated(w), residual=negated(res)), nb.rms_norm(x, w, residual=res)):
+            assert torch.equal(a, b)
+        assert torch.equal(nb.rms_norm(x, negated(w.to(torch.bfloat16))), nb.rms_norm(x, w.to(torch.bfloat16)))
+        for a, b in zip(nb.rms_norm_quantized(negated(x), negated(w)), nb.rms_norm_quantized(x, w)):
+            assert torch.equal(a.float(), b.float())
+    both = []
+    for mark in (negated, lambda t: t.clone()):
+        leaves = [mark(t).requires_grad_() for t in (x, w, res)]
+        y, r = nb.rms_norm(leaves[0], leaves[1], residual=leaves[2])
+        both.append(torch.autograd.grad([y, r], leaves, [mark(gy), mark(gr)]))
+    for a, b in zip(*both):
+        assert torch.equal(a, b)
