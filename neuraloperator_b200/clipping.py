@@ -14,6 +14,7 @@ from typing import Iterable, List, Sequence, Tuple, Union
 import torch
 
 from . import _lib
+from .utils import refuse_tangents
 
 _DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16,
            torch.complex64: _lib.DTYPE_FP32}
@@ -43,6 +44,7 @@ def _check(tensors: Sequence[torch.Tensor]) -> torch.device:
             raise TypeError(f"expected float32, bfloat16, float16 or complex64 tensors, got {dtype}")
     if len(devices) > 1:
         raise ValueError("all tensors must be on one device")
+    refuse_tangents(*tensors)
     return devices.pop()
 
 

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .utils import dense
+from .utils import dense, refuse_tangents
 
 _DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
@@ -68,6 +68,7 @@ def _check(x, w_gate, w_up, w_down, biases, activation, x_scale):
             raise TypeError("x_scale goes with a float8_e4m3fn field and bfloat16 or float16 weights")
         if x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (x.shape[0], 1, *x.shape[2:]):
             raise ValueError("x_scale must be float32 [batch, 1, *grid]")
+    refuse_tangents(x, w_gate, w_up, w_down, *biases, x_scale)
     return hidden, out
 
 

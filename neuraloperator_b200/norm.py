@@ -20,7 +20,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .utils import dense
+from .utils import dense, refuse_tangents
 
 _DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
@@ -42,6 +42,7 @@ def _check(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[t
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
                                  or residual.device != x.device):
         raise ValueError("residual must have x's shape, dtype and device")
+    refuse_tangents(x, weight, residual)
 
 
 def _desc(x: torch.Tensor, eps: float) -> _lib.NopNormDesc:

@@ -23,6 +23,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
+from .utils import refuse_tangents
 
 MAX_DIMS = 4
 
@@ -159,6 +160,7 @@ def chain(x: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor], w2: tor
     ``grad_relay``: under autograd, dL/dx is handed to that relay instead of returned (GradRelay)."""
     if not x.is_cuda:
         raise RuntimeError("neuraloperator_b200 runs on CUDA devices only (there is no CPU path)")
+    refuse_tangents(x, s, w0, w1, b1, w2, b2, gate_w, gate_b, w3, b3, w4, b4)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
                                        (x, s, w0, w1, b1, w2, b2, gate_w, gate_b, w3, b3, w4, b4)):
         if w3 is not None or w4 is not None:

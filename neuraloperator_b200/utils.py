@@ -6,6 +6,7 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 Number = Union[int, float]
 
@@ -46,6 +47,14 @@ def dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     if t.is_neg():
         return t.detach().resolve_neg().contiguous()
     return t if t.is_contiguous() and not t.requires_grad else t.detach().contiguous()
+
+
+def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Raises where one of the tensors carries a forward-mode tangent, for a call whose kernels read pointers alone: its
+    result would have none, a derivative of zero.  Outside a dual level there are no tangents and nothing is looked at."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode derivatives (torch.autograd.forward_ad) are not provided here")
 
 
 def count_model_params(model) -> int:
