@@ -210,7 +210,12 @@ class FNOBlocks(nn.Module):
                 skip = x_skip_mlp
         if self.norm is not None:
             norm = self.norm[self.n_norms * index + 1]
-            x = norm(x) if skip is None else norm(x, residual=skip)[0]
+            if skip is None:
+                x = norm(x)
+            elif x.dtype == skip.dtype:
+                x = norm(x, residual=skip)[0]
+            else:  # (autocast makes one of them 16 bits wide) the sum in the wider type
+                x = norm(x + skip)
         elif skip is not None:
             x = x + skip
         if not last:

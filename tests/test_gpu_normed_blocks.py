@@ -134,3 +134,21 @@ def test_training_steps_with_clipping():
         assert float(norm) > 1e-3
         assert abs(float(nb.global_norm([p.grad for p in model.parameters()])) - 1e-3) <= 1e-6
         opt.step()
+
+
+@pytest.mark.parametrize("kw", [dict(channel_mlp_type="gated", channel_mlp_skip="linear"), dict(),
+                                dict(channel_mlp_type="gated", preactivation=True)])
+def test_normed_models_under_autocast(kw):
+    """Autocast makes the torch layers' outputs bf16 and leaves this library's fp32: a skip of another type than the channel
+    MLP's output is added in the wider one."""
+    torch.manual_seed(0)
+    model = nb.FNO(n_modes=(8, 8), in_channels=1, out_channels=1, hidden_channels=16, n_layers=2, norm="rms_norm",
+                   **kw).cuda()
+    x = torch.randn(2, 1, 16, 20, device="cuda")
+    want = model(x)
+    with torch.autocast("cuda", torch.bfloat16):
+        y = model(x)
+    # a dozen torch layers in a row round to bf16, 2^-8 each, and every gain is of the order of one
+    assert rel(y, want.cpu()) <= 12 * 2.0 ** -8
+    y.float().square().mean().backward()
+    assert all(torch.isfinite(torch.view_as_real(p.grad) if p.is_complex() else p.grad).all() for p in model.parameters())
