@@ -71,7 +71,8 @@ class FNOBlocks(nn.Module):
                                       "complex data on its own")
         if norm not in (None, "rms_norm"):
             raise NotImplementedError(f"norm={norm!r} is not provided (None, the FNO default, or 'rms_norm')")
-        self.n_norms = 2
+        # a preactivation block has its second norm before the channel MLP: without one, a parameter that nothing uses
+        self.n_norms = 1 if preactivation and not use_channel_mlp else 2
         self.norm = (nn.ModuleList([RMSNorm(out_channels) for _ in range(self.n_norms * n_layers)])
                      if norm == "rms_norm" else None)
         if preactivation and norm == "rms_norm" and in_channels != out_channels:

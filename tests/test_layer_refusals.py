@@ -205,3 +205,18 @@ def test_block_options():
     with pytest.raises(RuntimeError, match="CUDA"):
         model(fake(1, 1, 8, 8))
     assert nb.FNO(**kw).fno_blocks.norm is None  # the default is as it was
+
+
+@pytest.mark.parametrize("preactivation", [False, True])
+@pytest.mark.parametrize("use_channel_mlp", [False, True])
+def test_every_norm_is_used(preactivation, use_channel_mlp, monkeypatch):
+    """Each layer's forward calls all of its norms, and no other's."""
+    blocks = nb.FNOBlocks(4, 4, (2, 2), n_layers=2, norm="rms_norm", preactivation=preactivation,
+                          use_channel_mlp=use_channel_mlp)
+    called = []
+    monkeypatch.setattr(nb.RMSNorm, "forward", lambda self, x, residual=None: (
+        called.append(id(self)), x if residual is None else (x + residual, x))[1])
+    monkeypatch.setattr(nb.SpectralConv, "forward", lambda self, x, output_shape=None: x)
+    for index in range(2):
+        blocks(torch.zeros(1, 4, 4, 4), index)
+    assert called == [id(m) for m in blocks.norm]
