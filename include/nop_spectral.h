@@ -477,7 +477,8 @@ typedef struct nop_gated_grads {
     void* gb_down;
 } nop_gated_grads;
 
-/* workspace: device memory, 256-byte aligned, of the size for the pass (backward: 0 or 1). */
+/* workspace: device memory, 256-byte aligned, of the size for the pass (backward: 0, 1, or 2 for dL/dx alone).  The weights'
+ * gradients take up to 512 MB, more where a hidden width above some 2300 needs it (3.8 GB at 16384). */
 int32_t nop_gated_workspace_size(const nop_gated_desc* desc, int32_t backward, size_t* bytes);
 int32_t nop_gated_forward(const nop_gated_desc* desc, const nop_gated_operands* operands, void* workspace,
                           size_t workspace_bytes, void* stream);

@@ -1716,8 +1716,9 @@ struct Sizes {
     int splits, wtiles;
 };
 
+// weights: the backward leaves gradients of the weights or the biases, beside or without dL/dx
 template <class T>
-Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd) {
+Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd, bool weights) {
     auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
     Sizes s{};
     s.tiles = ceil_div(d.batch * d.points, TP);
@@ -1731,8 +1732,9 @@ Sizes sizes_of(const nop_gated_desc& d, const Plan& p, bool bwd) {
     at += up(images);
     s.vec = at;
     at += up(vectors);
-    if (bwd) {
-        // The scratch of a slab: up to 512 MB, in whole waves of 148 tiles.  Slabs that stay in L2 save the scratch's
+    if (weights) {
+        // The scratch of a slab: up to 512 MB, in whole waves of 148 tiles, and at least one wave (512 MB at a hidden width of
+        // some 2300, 3.8 GB at 16384 with 256 channels).  Slabs that stay in L2 save the scratch's
         // trip through HBM but lose more to their launches' beginnings and ends: 64 MB slabs took 2207 us where
         // 512 MB take 1646 (fp32, 64 channels, hidden 128, 2^20 points), and larger ones 1626.
         using Z = typename Scratch<T>::type;
@@ -1876,6 +1878,10 @@ int32_t forward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, co
     }
 }
 
+bool of_weights(const nop_gated_grads& g) {
+    return g.gw_gate || g.gw_up || g.gw_down || g.gb_gate || g.gb_up || g.gb_down;
+}
+
 template <class T>
 int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, const nop_gated_grads& g,
                  const Sizes& z, char* ws, cudaStream_t s) {
@@ -1883,7 +1889,7 @@ int32_t backward(const nop_gated_desc& d, Plan p, const nop_gated_operands& o, c
     int32_t rc = device(&dev);
     if (rc != NOP_OK) return rc;
     if ((rc = pack<T, true>(p, o, z, ws, s)) != NOP_OK) return rc;
-    const bool weights = g.gw_gate || g.gw_up || g.gw_down || g.gb_gate || g.gb_up || g.gb_down;
+    const bool weights = of_weights(g);
     Params q = params_of<T>(d, p, o, z, ws);
     q.gy = g.gy;
     q.out = g.gx;
@@ -1982,12 +1988,13 @@ int32_t nop_gated_workspace_size(const nop_gated_desc* d, int32_t backward, size
     const int32_t rc = gated::check(d);
     if (rc != NOP_OK) return rc;
     if (!bytes) return fail(NOP_E_INVALID, "bytes is NULL");
+    if (backward < 0 || backward > 2) return fail(NOP_E_INVALID, "the pass must be 0, 1 or 2");
     return gated::by_type(d->dtype, [&](auto t) {
         using T = decltype(t);
         gated::Plan p;
         if (!gated::make_plan<T>(*d, backward != 0, 0, &p))
             return fail(NOP_E_UNSUPPORTED, gated::kTooLarge);
-        *bytes = gated::sizes_of<T>(*d, p, backward != 0).bytes;
+        *bytes = gated::sizes_of<T>(*d, p, backward != 0, backward == 1).bytes;
         return (int32_t)NOP_OK;
     });
 }
@@ -2004,7 +2011,7 @@ int32_t nop_gated_forward(const nop_gated_desc* d, const nop_gated_operands* o, 
         gated::Plan p;
         if (!gated::make_plan<T>(*d, false, 0, &p))
             return fail(NOP_E_UNSUPPORTED, gated::kTooLarge);
-        const gated::Sizes z = gated::sizes_of<T>(*d, p, false);
+        const gated::Sizes z = gated::sizes_of<T>(*d, p, false, false);
         if (!workspace || workspace_bytes < z.bytes) return fail(NOP_E_WORKSPACE, "workspace missing or too small");
         if ((uintptr_t)workspace % 256) return fail(NOP_E_ALIGNMENT, "the workspace must be 256-byte aligned");
         char* ws = static_cast<char*>(workspace);
@@ -2041,7 +2048,7 @@ int32_t nop_gated_backward(const nop_gated_desc* d, const nop_gated_operands* o,
         gated::Plan p;
         if (!gated::make_plan<T>(*d, true, 0, &p))
             return fail(NOP_E_UNSUPPORTED, gated::kTooLarge);
-        const gated::Sizes z = gated::sizes_of<T>(*d, p, true);
+        const gated::Sizes z = gated::sizes_of<T>(*d, p, true, gated::of_weights(*g));
         if (!workspace || workspace_bytes < z.bytes) return fail(NOP_E_WORKSPACE, "workspace missing or too small");
         if ((uintptr_t)workspace % 256) return fail(NOP_E_ALIGNMENT, "the workspace must be 256-byte aligned");
         return gated::backward<T>(*d, p, *o, *g, z, static_cast<char*>(workspace), s);

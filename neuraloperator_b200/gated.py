@@ -117,7 +117,7 @@ class _GatedFn(torch.autograd.Function):
         grads = [torch.empty(t.shape, device=x.device, dtype=t.dtype) if t is not None and need else None
                  for t, need in zip(saved, ctx.needs_input_grad)]
         lib, desc = _lib.library(), _desc(x, w_gate.dtype, hidden, out, activation)
-        ws = _workspace(lib, desc, 1, x.device)
+        ws = _workspace(lib, desc, 1 if any(t is not None for t in grads[1:]) else 2, x.device)
         ops = _lib.NopGatedOperands(_ptr(x), None, _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(b_gate), _ptr(b_up),
                                     _ptr(b_down), None)
         g = _lib.NopGatedGrads(gy.data_ptr(), *[_ptr(t) for t in grads])

@@ -207,6 +207,24 @@ def test_block_options():
     assert nb.FNO(**kw).fno_blocks.norm is None  # the default is as it was
 
 
+def test_gated_workspace_of_a_part():
+    """dL/dx alone takes the packed weights and no scratch of the points; the backward checks what it is given."""
+    lib, size = _lib.library(), ctypes.c_size_t()
+    for dtype in range(3):
+        sizes = {}
+        for points in (16, 1 << 20):
+            d = gated_desc(dtype=dtype, x_dtype=dtype, points=points)
+            for which in (0, 1, 2):
+                assert lib.nop_gated_workspace_size(d, which, size) == 0
+                sizes[points, which] = size.value
+        assert sizes[16, 2] == sizes[1 << 20, 2] < sizes[16, 1] < sizes[1 << 20, 1]
+        ops = _lib.NopGatedOperands(x=512, w_gate=512, w_up=512, w_down=512)
+        back = lambda n, **g: lib.nop_gated_backward(d, ops, _lib.NopGatedGrads(gy=512, **g), 512, n, None)  # noqa: E731
+        assert back(sizes[1 << 20, 2], gx=512, gb_up=512) == -4 and back(sizes[1 << 20, 2] - 1, gx=512) == -4
+    assert lib.nop_gated_workspace_size(gated_desc(), 3, size) == -1
+    assert lib.nop_gated_workspace_size(gated_desc(), -1, size) == -1
+
+
 @pytest.mark.parametrize("preactivation", [False, True])
 @pytest.mark.parametrize("use_channel_mlp", [False, True])
 def test_every_norm_is_used(preactivation, use_channel_mlp, monkeypatch):
