@@ -204,3 +204,18 @@ def test_gates_far_below_zero_are_shut(gate, act):
 def test_huge_gates_leave_their_neighbours(gate, act):
     """Gates whose products overflow fp32 share a reciprocal with small ones."""
     check_huge(gate, act)
+
+
+# 148 tiles of a slab at a hidden width of 2400; 3996 tiles (fp32 scratch) and 4588 (two bf16 parts) at 64 with 64 channels
+# in all: the last slab has fewer pieces than the points' splits
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", ["wide odd", "wide whole", "long odd", "long whole"])
+def test_several_slabs(shape, dtype):
+    """The backward's scratch is made and consumed slab by slab: sums that go on over two of them, the last one short, with
+    the fields copied to the scratch (odd rows) and read in place (samples of whole tiles, one of them across the slabs)."""
+    tiles = 4588 if dtype == torch.bfloat16 else 3996
+    batch, c, h, o, grid = {"wide odd": (2, 20, 2400, 12, (12501,)), "wide whole": (2, 20, 2400, 12, (98, 128)),
+                            "long odd": (1, 32, 64, 32, (tiles * 128 + 597,)),
+                            "long whole": (2, 32, 64, 32, ((tiles + 6) // 2, 128))}[shape]
+    check(operands(batch, c, h, o, grid, dtype, seed=21), "silu")

@@ -277,3 +277,37 @@ def test_lazily_negated_tensors(dtype):
         both.append(torch.autograd.grad([y, r], leaves, [mark(gy), mark(gr)]))
     for a, b in zip(*both):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels", [24, 72, 128, 160, 256, 300])
+@pytest.mark.parametrize("points", [76000, 76004, 76002])  # 8, 4 and 2 values a thread, forward; 4, 4 and 2 backward
+def test_wide_rows_of_many_channels(channels, points, dtype):
+    """Every channel class at every vector width: y, the sum, the 8-bit output and the gradients, with a residual."""
+    shape = (1, channels, points)
+    x, w, res = make(shape, dtype, 1, 1.5), make((channels,), torch.float32, 2), make(shape, dtype, 3)
+    gy, gr = make(shape, dtype, 4), make(shape, dtype, 5)
+    u, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal
+    leaves = [t.clone().requires_grad_() for t in (x, res, w)]
+    y, r = nb.rms_norm(leaves[0], leaves[2], residual=leaves[1], eps=EPS)
+    gx, gres, gw = torch.autograd.grad([y, r], leaves, [gy, gr])
+    with torch.no_grad():
+        y64, r64, inv = define(x, w, res)
+        assert torch.equal(r.double(), r64) and torch.equal(gx, gres)
+        assert ((y.double() - y64).abs() <= y_bound(y64, channels, dtype)).all()
+        y0, _, _ = define(x, w, None)
+        assert ((nb.rms_norm(x, w, eps=EPS).double() - y0).abs() <= y_bound(y0, channels, dtype)).all()
+        q, s, r = nb.rms_norm_quantized(x, w, residual=res, eps=EPS)
+        assert torch.equal(r.double(), r64)
+        # e4m3: half a step of three bits after the first, 2^-10 of the scale below its smallest normal number
+        off = (q.double() * s.double() - y64).abs()
+        assert (off <= y64.abs() * (2.0 ** -4 + (channels / 2 + 8) * V) + s.double() * 2.0 ** -10).all()
+        del q, s, off, y0
+        g, wv = gy.double(), w.double().view(1, -1, 1)
+        hat = r64 * inv
+        m, m_abs = (g * wv * hat).mean(1, keepdim=True), (g * wv * hat).abs().mean(1, keepdim=True)
+        want = inv * (g * wv - hat * m) + gr.double()
+        size = inv * ((g * wv).abs() + hat.abs() * m_abs) + gr.double().abs()
+        assert ((gx.double() - want).abs() <= want.abs() * u + size * (2 * channels + 16) * V + tiny).all()
+        want, size = (g * hat).sum([0, 2]), (g * hat).abs().sum([0, 2])
+        assert ((gw.double() - want).abs() <= size * (points / 32 + channels / 2 + 64) * V).all()
