@@ -433,8 +433,9 @@ int32_t nop_rms_norm_backward(const nop_norm_desc* desc, const void* r, const fl
  * At every point of x [batch, channels, points]:
  *   h = act(w_gate x + b_gate) * (w_up x + b_up),  y = w_down h + b_down      y [batch, out_channels, points]
  * w_gate, w_up [hidden, channels], w_down [out_channels, hidden], biases (each may be NULL) [hidden], [hidden],
- * [out_channels], all of the field's type `dtype`.  fp32 in fp32 accuracy; 16-bit types with fp32 sums and h to
- * twice the type's precision.  x_dtype: dtype, or NOP_DTYPE_E4M3 (forward only, 16-bit dtype) with x_scale [batch, points]
+ * [out_channels], all of the field's type `dtype`.  fp32: within about 1e-6 of the results' size at up to 64
+ * channels, 4e-6 at 256.  16-bit types: fp32 sums, h in two parts of the type (fp16: in its range, down to 2^-24), and so
+ * dg and du, dL/d(w_gate x + b_gate) and dL/d(w_up x + b_up), on their way into dL/dx.  x_dtype: dtype, or NOP_DTYPE_E4M3 (forward only, 16-bit dtype) with x_scale [batch, points]
  * float32, the values being x * x_scale.  Values that are not finite, h among them (fp16: above 65504),
  * give results that are not finite at their point.  channels and out_channels <= 256, hidden <= 16384, fewer than 2^31 points. */
 typedef enum nop_activation { NOP_ACT_SILU = 0, NOP_ACT_GELU = 1 } nop_activation;

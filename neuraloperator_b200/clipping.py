@@ -2,7 +2,8 @@
 ``loss.backward()`` and ``optimizer.step()``.
 
 Tensors are float32, bfloat16, float16 or complex64 (the spectral weights; a complex value counts as its real and
-imaginary part), on one CUDA device.  No call synchronises with the host, and the sums do not depend on scheduling.
+imaginary part), on one CUDA device.  No call synchronises with the host, and the sums do not depend on scheduling.  Squares
+are float32: a value above 1.8e19 makes the 2-norm infinite, and values below 1e-22 do not count in it.
 """
 
 from __future__ import annotations

@@ -20,13 +20,16 @@
 // Operands.  16-bit fields multiply as they are (products exact, fp32 sums); h, dg and du go into their products in two
 // 16-bit parts (Mid), and into the weights' gradients in two bf16 parts or in fp32 (Scratch).  fp32 values are split into three
 // bf16 parts, v = a + b + c to within 2^-26 |v|, and six of the nine products are summed (the three left out are
-// below 2^-26): fp32 accuracy at the cost of six 16-bit MMAs, the same tensor time as three tf32 passes on a
+// below 2^-26): near fp32 accuracy at the cost of six 16-bit MMAs, the same tensor time as three tf32 passes on a
 // hi / lo split but three quarters of its shared memory, and 2^-26 instead of 2^-21.  The tensor core adds to its
 // accumulator with truncation, about 2^-25 of it towards zero every time, so the five smaller products, 2^-8 of the
 // first and less, are kept from the large accumulator: the second product gives them columns of their own (D2c,
 // added at the end), the first product adds them before the large one, piece by piece.  (All six into one
-// accumulator: dL/dx was 4.7e-6 off at 128 channels, hidden 200.)  An e4m3 field is widened exactly and its point's
-// scale multiplies the accumulator.
+// accumulator: dL/dx was 4.7e-6 off at 128 channels, hidden 200.)  From the second piece on they meet a large D1 all the
+// same, for which tensor memory has no second set of columns: outputs are 0.5 to 1.1e-6 of their size off float64 at up to
+// 64 channels, 1.8e-6 at 128 and 3.6e-6 at 256 (fp32 products: 0.3 to 0.9e-6).  fp16: h, and dg and du on their way into
+// dL/dx, have fp16's range and its smallest step, 2^-24.  An e4m3 field is widened exactly and its point's scale multiplies
+// the accumulator.
 //
 // The points of a channel are contiguous and the MMA wants a point's channels contiguous (K-major core matrices of
 // 8 rows x 16 bytes): a producer thread loads 8 channels x 4 points with one wide load a channel and writes four
@@ -49,9 +52,10 @@
 // their arithmetic, both operands coming from shared memory, the second one's (N = 64) 50; the middle takes 1650 cycles
 // of a job's 4050.  A third D1 buffer, more weights or pieces of x in flight, or MMAs issued in blocks changed nothing.
 // 16-bit types are bound by the middle (800 cycles for 16 hidden channels of a warp's points; exponentials, reciprocals
-// and conversions): bf16 128 / 384 / 128 on 32 fields of 85 x 85, rows not aligned, 150 us forward and 480 us backward
-// (products alone: 41 and 110 us).  In the backward the scratch's stores lengthen the middle to 4400 cycles a job, and
-// k_wgrad reads it at 4.6 TB/s.  Pairs of CTAs (cta_group::2, half of the weights in each) ran slower at nearly all
+// and conversions): bf16 128 / 384 / 128 on 32 fields of 85 x 85, rows not aligned, 153 us forward and 684 us backward
+// (products alone: 41 and 110 us); 64 / 128 / 64 on 2^20 points 182 and 915 us, fp16 184 and 1052.  In the backward the
+// scratch's stores lengthen the middle (to 4400 cycles a job with dg, du and h rounded to one part, whose bytes were half:
+// 484 and 557 us), and k_wgrad reads it at 4.6 TB/s.  Pairs of CTAs (cta_group::2, half of the weights in each) ran slower at nearly all
 // sizes (fp32 forward above 548 us, bf16 32 / 32 / 32 121 us against 70).
 //
 // Every wait is bounded: on expiry the kernel records NOP_DEVICE_MMA_TIMEOUT in the status word, all roles leave

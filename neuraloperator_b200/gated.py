@@ -131,9 +131,10 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
               x_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y [batch, out, *grid] (see the module docstring).  x: a field [batch, channels, *grid] on a CUDA device;
     w_gate, w_up: [hidden, channels], w_down: [out, hidden] (or Conv1d weights [., ., 1]); biases [hidden], [hidden],
-    [out] or None; all of x's dtype: float32 (fp32 accuracy), bfloat16 or float16 (fp32 sums).  activation: "silu" or
-    "gelu" (exact).  channels and out <= 256, hidden <= 16384.  The hidden values have the dtype's range (float16: a
-    hidden value above 65504 makes its point's output not finite).
+    [out] or None; all of x's dtype: float32 (within about 1e-6 of the results' size at up to 64 channels, 4e-6 at 256),
+    bfloat16 or float16 (fp32 sums, results rounded once).  activation: "silu" or "gelu" (exact).  channels and out <= 256,
+    hidden <= 16384.  The hidden values, and their gradients on the way into dL/dx, have the dtype's range (float16: one
+    above 65504 makes its point's output not finite, and 2^-24 is the smallest step).
 
     With ``x_scale`` (float32 [batch, 1, *grid]) x is float8_e4m3fn and stands for x * x_scale, as
     ``rms_norm_quantized`` leaves it; weights and output are bfloat16 or float16 (inference only).

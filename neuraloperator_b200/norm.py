@@ -118,7 +118,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     """y, or (y, x + residual) with a residual (see the module docstring).  x: a float32, bfloat16 or float16 field
     [batch, channels, *grid] on a CUDA device; residual: the same shape and dtype; weight: [channels], any
     floating-point dtype (None: ones).  The sum is rounded to x's dtype before it is normed; the statistics are
-    float32.  Runs on x's device and its current stream."""
+    float32 (values above 1.8e19 have an infinite square).  Runs on x's device and its current stream."""
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         return _RMSNormFn.apply(x, weight, residual, eps)
